@@ -39,6 +39,14 @@ typedef void* st_stream_t; /* hipStream_t */
 #define ST_POOL_FLOOR 0 /* torchvision vgg19 MaxPool2d(2,2), trainer.py:168 */
 #define ST_POOL_CEIL 1  /* MaxPool2d((2,2),(2,2),(0,0),ceil_mode=True), generator.py:53,60,73 */
 
+#define ST_F32 0 /* storage type of logits and of their gradient */
+#define ST_BF16 1
+#define ST_F16 2
+
+#define ST_PREF_SIGMOID 0 /* -(1-eps) ln sigmoid(z) - eps ln sigmoid(-z), z = beta h */
+#define ST_PREF_IPO 1     /* (h - 1 / (2 beta))^2 */
+#define ST_PREF_HINGE 2   /* max(0, 1 - z) */
+
 #define ST_HIST_INVERSE_QUADRATIC 0 /* losses.py:228-234 */
 #define ST_HIST_RBF 1               /* losses.py:221-227 */
 #define ST_HIST_THRESHOLDING 2      /* losses.py:218-220 */
@@ -475,6 +483,62 @@ int st_aug_color_jitter_slot(const float* x, float* y, const int* code_dev, cons
                              float* gray_mean_ws, int n, int hw, st_stream_t stream);
 /* transforms.RandomHorizontalFlip: flip_dev[i] != 0 = flip. */
 int st_aug_hflip(const float* x, float* y, const int* flip_dev, int n, int c, int h, int w, st_stream_t stream);
+
+/* ---- losses over rows of logits (csrc/token_losses.hip; no counterpart in the reference) -------------------------
+ * Logits: `rows` rows of `vocab` elements of `dtype` (ST_F32 / ST_BF16 / ST_F16), last stride 1, row r at
+ * (r / inner) * s_outer + (r % inner) * s_inner elements; any alignment of the type.  Gradients: contiguous
+ * [rows][vocab] of the same type, every row written.  Labels [rows], int64 (labels64) or int32; a row whose label
+ * is `ignore` does not count: its logits are not read, its results and its gradient row are 0.  A label outside
+ * [0, vocab) makes its row NaN.  tau: temperature.  Sequences of a packed batch: cu_seqlens int32 [count + 1],
+ * ascending row numbers (rows outside it do not count); of a padded one (cu_seqlens NULL): `inner` rows each.
+ * `scale` multiplies a loss and its gradient.  Every result is the same from run to run.
+ *
+ * logp[r] = ln softmax(x / tau)[label], entropy[r] (may be NULL) of the same distribution; state [rows][4] (may be
+ * NULL) is what the backward pass needs.  g_logp / g_entropy: the rows' upstream gradients (either may be NULL). */
+size_t st_token_workspace_bytes(int dtype, long long rows, int vocab, long long sequences);
+int st_token_logprobs_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
+                          long long s_inner, int vocab, const void* labels, int labels64, int ignore, double tau,
+                          float* logp, float* entropy, float* state, void* workspace, st_stream_t stream);
+int st_token_logprobs_bwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
+                          long long s_inner, int vocab, const void* labels, int labels64, int ignore, double tau,
+                          const float* state, const float* g_logp, const float* g_entropy, void* grad,
+                          st_stream_t stream);
+/* Preference loss of 2 * pairs sequences, the chosen ones first: h = (L_c - ref_c) - (L_r - ref_r) with L the sum
+ * (average: the mean) of a sequence's log-probabilities, ref_logps [2 * pairs] or NULL; mean over the pairs.
+ * rewards [2 * pairs]: beta (L - ref) of each sequence.  row_grad [rows][4] (NULL: no gradient follows). */
+int st_preference_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
+                           long long s_inner, int vocab, const void* labels, int labels64, int ignore,
+                           const int* cu_seqlens, int pairs, const float* ref_logps, int kind, int average,
+                           double beta, double label_smoothing, double scale, float* loss, float* rewards,
+                           float* row_grad, void* workspace, st_stream_t stream);
+/* Clipped policy loss: r = exp(logp - old), s = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A),
+ * k = exp(ref - logp) - (ref - logp) - 1 (ref_logps NULL: 0), mean of s + kl_coef k - entropy_coef H over the tokens, or
+ * (per_sequence) over the sequences of the mean over a sequence's tokens.  old_logps, ref_logps [rows]; advantages [rows]
+ * or (adv_per_sequence) [sequences].  stats [4]: the same mean of s, k, H and of "the clip holds r". */
+int st_policy_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
+                       long long s_inner, int vocab, const void* labels, int labels64, int ignore, double tau,
+                       const int* cu_seqlens, int sequences, const float* old_logps, const float* advantages,
+                       int adv_per_sequence, const float* ref_logps, double clip_low, double clip_high,
+                       double kl_coef, double entropy_coef, int per_sequence, double scale, float* loss,
+                       float* stats, float* row_grad, void* workspace, st_stream_t stream);
+/* grad = gout[0] (NULL: 1) times the gradient of the preference or the policy loss, from their row_grad. */
+int st_token_loss_bwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
+                      long long s_inner, int vocab, const void* labels, int labels64, int ignore, double tau,
+                      const float* row_grad, const float* gout, void* grad, st_stream_t stream);
+/* Distillation from a teacher's top logits: teacher_idx [rows][k] (int64: idx64, or int32; below 0: unused),
+ * teacher_val [rows][k]; mask [rows] (NULL: all rows) says which rows count, loss = tau^2 times their mean of
+ * sum p (ln p - ln q).  tail = 0: p = softmax(val / tau) over the list.  tail = 1: p = exp(val), and what the teacher
+ * and the student have off the list is one more bucket.  An index >= vocab makes its row NaN; entries with the same
+ * index add up.  row_grad [rows][8] (NULL: no gradient follows). */
+size_t st_distill_workspace_bytes(int dtype, long long rows, int vocab);
+int st_distill_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
+                        long long s_inner, int vocab, const void* teacher_idx, int idx64, const float* teacher_val,
+                        int k, const unsigned char* mask, double tau, int tail, double scale, float* loss,
+                        float* row_grad, void* workspace, st_stream_t stream);
+int st_distill_loss_bwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
+                        long long s_inner, int vocab, const void* teacher_idx, int idx64, const float* teacher_val,
+                        int k, double tau, int tail, const float* row_grad, const float* gout, void* grad,
+                        st_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -7,12 +7,16 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_longlong, c_size_t, c_void_p
+from ctypes import c_double, c_float, c_int, c_longlong, c_size_t, c_void_p
 
 import torch
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libst_hip.so")
+
+# argument groups of the losses over rows of logits
+_LOGITS = [c_void_p, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_int]   # x, dtype, rows, inner, strides, vocab
+_LABELS = [c_void_p, c_int, c_int]                                                  # labels, int64?, ignore
 
 # name -> (restype, argtypes); every symbol include/st_hip.h declares
 SIGNATURES = {
@@ -123,6 +127,20 @@ SIGNATURES = {
     "st_aug_sharpness": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "st_aug_color_jitter_slot": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "st_aug_hflip": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    "st_token_workspace_bytes": (c_size_t, [c_int, c_longlong, c_int, c_longlong]),
+    "st_token_logprobs_fwd": (c_int, [*_LOGITS, *_LABELS, c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "st_token_logprobs_bwd": (c_int, [*_LOGITS, *_LABELS, c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "st_preference_loss_fwd": (c_int, [*_LOGITS, *_LABELS, c_void_p, c_int, c_void_p, c_int, c_int, c_double, c_double, c_double,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "st_policy_loss_fwd": (c_int, [*_LOGITS, *_LABELS, c_double, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_double,
+                                   c_double, c_double, c_double, c_int, c_double, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p]),
+    "st_token_loss_bwd": (c_int, [*_LOGITS, *_LABELS, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "st_distill_workspace_bytes": (c_size_t, [c_int, c_longlong, c_int]),
+    "st_distill_loss_fwd": (c_int, [*_LOGITS, c_void_p, c_int, c_void_p, c_int, c_void_p, c_double, c_int, c_double, c_void_p,
+                                    c_void_p, c_void_p, c_void_p]),
+    "st_distill_loss_bwd": (c_int, [*_LOGITS, c_void_p, c_int, c_void_p, c_int, c_double, c_int, c_void_p, c_void_p, c_void_p,
+                                    c_void_p]),
     "st_syevj_small_max_dim": (c_int, []),
     "st_syevj_small_batched": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
 }

@@ -13,6 +13,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib, ops
+from .token_losses import (ClippedPolicyLoss, PolicyOutput, PreferenceLoss, PreferenceOutput, TokenLogProbs,  # noqa: F401
+                           TopKDistillLoss, clipped_policy_loss, preference_loss, token_logprobs, topk_distill_loss)
 
 
 def _workspace(dev):
