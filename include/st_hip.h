@@ -514,31 +514,34 @@ int st_preference_loss_fwd(const void* x, int dtype, long long rows, long long i
 /* Clipped policy loss: r = exp(logp - old), s = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A),
  * k = exp(ref - logp) - (ref - logp) - 1 (ref_logps NULL: 0), mean of s + kl_coef k - entropy_coef H over the tokens, or
  * (per_sequence) over the sequences of the mean over a sequence's tokens.  old_logps, ref_logps [rows]; advantages [rows]
- * or (adv_per_sequence) [sequences].  stats [4]: the same mean of s, k, H and of "the clip holds r". */
+ * or (adv_per_sequence) [sequences].  grad (may be NULL): the gradient of loss, written in the same pass; row_grad [rows][4]
+ * (may be NULL) lets st_token_loss_bwd compute it again.  stats [4]: the same mean of s, k, H and of "the clip holds r". */
 int st_policy_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
                        long long s_inner, int vocab, const void* labels, int labels64, int ignore, double tau,
                        const int* cu_seqlens, int sequences, const float* old_logps, const float* advantages,
                        int adv_per_sequence, const float* ref_logps, double clip_low, double clip_high,
                        double kl_coef, double entropy_coef, int per_sequence, double scale, float* loss,
-                       float* stats, float* row_grad, void* workspace, st_stream_t stream);
-/* grad = gout[0] (NULL: 1) times the gradient of the preference or the policy loss, from their row_grad. */
+                       float* stats, float* row_grad, void* grad, void* workspace, st_stream_t stream);
+/* grad = gout[0] (NULL: 1) times the gradient of the preference or the policy loss, from their row_grad.
+ * grad_is_for_one: grad holds the gradient for an upstream gradient of 1 already (st_policy_loss_fwd wrote it), and stays
+ * as it is where gout[0] == 1. */
 int st_token_loss_bwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
                       long long s_inner, int vocab, const void* labels, int labels64, int ignore, double tau,
-                      const float* row_grad, const float* gout, void* grad, st_stream_t stream);
+                      const float* row_grad, const float* gout, int grad_is_for_one, void* grad, st_stream_t stream);
 /* Distillation from a teacher's top logits: teacher_idx [rows][k] (int64: idx64, or int32; below 0: unused),
  * teacher_val [rows][k]; mask [rows] (NULL: all rows) says which rows count, loss = tau^2 times their mean of
  * sum p (ln p - ln q).  tail = 0: p = softmax(val / tau) over the list.  tail = 1: p = exp(val), and what the teacher
  * and the student have off the list is one more bucket.  An index >= vocab makes its row NaN; entries with the same
  * index add up.  row_grad [rows][8] (NULL: no gradient follows). */
-size_t st_distill_workspace_bytes(int dtype, long long rows, int vocab);
+size_t st_distill_workspace_bytes(long long rows);
 int st_distill_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
                         long long s_inner, int vocab, const void* teacher_idx, int idx64, const float* teacher_val,
                         int k, const unsigned char* mask, double tau, int tail, double scale, float* loss,
-                        float* row_grad, void* workspace, st_stream_t stream);
+                        float* row_grad, void* grad, void* workspace, st_stream_t stream);
 int st_distill_loss_bwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
                         long long s_inner, int vocab, const void* teacher_idx, int idx64, const float* teacher_val,
-                        int k, double tau, int tail, const float* row_grad, const float* gout, void* grad,
-                        st_stream_t stream);
+                        int k, double tau, int tail, const float* row_grad, const float* gout, int grad_is_for_one,
+                        void* grad, st_stream_t stream);
 
 #ifdef __cplusplus
 }

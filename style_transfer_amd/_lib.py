@@ -134,13 +134,13 @@ SIGNATURES = {
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "st_policy_loss_fwd": (c_int, [*_LOGITS, *_LABELS, c_double, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_double,
                                    c_double, c_double, c_double, c_int, c_double, c_void_p, c_void_p, c_void_p, c_void_p,
-                                   c_void_p]),
-    "st_token_loss_bwd": (c_int, [*_LOGITS, *_LABELS, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "st_distill_workspace_bytes": (c_size_t, [c_int, c_longlong, c_int]),
+                                   c_void_p, c_void_p]),
+    "st_token_loss_bwd": (c_int, [*_LOGITS, *_LABELS, c_double, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "st_distill_workspace_bytes": (c_size_t, [c_longlong]),
     "st_distill_loss_fwd": (c_int, [*_LOGITS, c_void_p, c_int, c_void_p, c_int, c_void_p, c_double, c_int, c_double, c_void_p,
-                                    c_void_p, c_void_p, c_void_p]),
-    "st_distill_loss_bwd": (c_int, [*_LOGITS, c_void_p, c_int, c_void_p, c_int, c_double, c_int, c_void_p, c_void_p, c_void_p,
-                                    c_void_p]),
+                                    c_void_p, c_void_p, c_void_p, c_void_p]),
+    "st_distill_loss_bwd": (c_int, [*_LOGITS, c_void_p, c_int, c_void_p, c_int, c_double, c_int, c_void_p, c_void_p, c_int,
+                                    c_void_p, c_void_p]),
     "st_syevj_small_max_dim": (c_int, []),
     "st_syevj_small_batched": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
 }

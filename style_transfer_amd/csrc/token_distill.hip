@@ -1,0 +1,421 @@
+// Distillation from a teacher's top logits for gfx950 (token_rows.h: the row kernels' shared code).  HBM-bound.
+//
+// The list of a row is K pairs (index, value); an index below 0 is unused.  p_k is the teacher's probability of entry k,
+// P their sum, and with a bucket for all that is not listed rest = max(0, 1 - P) and q_rest the student's mass off the list:
+//   loss / tau^2 = sum p_k (ln p_k - ln q_k) + rest (ln rest - ln q_rest)
+//   d / dx_j = tau (Q q_j - p_j) on the list,  tau q_j (Q - rest / q_rest) off it,  Q = P + rest
+// q_rest comes from its own sum over the elements off the list (a bitmap in LDS tells them apart): 1 - sum q_k would keep
+// no digit of it where the student is sure of a listed token.  Entries that name the same token add up.
+//
+// A first kernel takes what the lists alone say (a wave a row, in fp64, K values and K gathered logits); the second holds a
+// row in registers, with -inf in place of the listed elements, so that its statistics are those off the list, and writes
+// the gradient in two steps: the stream as if nothing were listed, then the K entries over it.
+#include "token_rows.h"
+
+namespace {
+
+using namespace st_token;
+
+constexpr int MAX_VOCAB = 1 << 20;       // the bitmap of a row: 128 KB of LDS
+constexpr size_t MAX_PLAIN_LDS = 48 << 10;   // dynamic LDS that a kernel gets without asking (64 KB with what it declares)
+
+// what the list of a row says by itself
+struct ListSum {
+  double m, s, w;            // the listed logits' maximum, and S and W of the listed tokens seen from it (once each entry)
+  double vref, z;            // the values' maximum and sum of exp((v - vref) / tau); tail: 0 and unused
+  double mass, plogp, px;    // P, sum p ln p, sum p (x - m) / tau
+  double used;               // entries
+  double bad;                // an index outside the vocabulary
+};
+
+struct ListIn {
+  const void* idx;           // [rows][k] int64 or int32
+  int idx64;
+  const float* val;          // [rows][k]
+  int k;
+  const unsigned char* mask; // [rows] or null
+  int tail;
+  double scale;
+  ListSum* sum;              // [rows]
+  f32x4* row;                // [rows][2]: (m_off, alpha_off, m, alpha_on), (vref, g / Z, an index twice, not zero) or null
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
+}
+
+// index of entry k: -1 unused, -2 outside the vocabulary
+__device__ __forceinline__ int entry_index(const ListIn& q, size_t at, int vocab) {
+  const long long j = load_index(q.idx, q.idx64, at);
+  return j < 0 ? -1 : j >= vocab ? -2 : (int)j;
+}
+
+// A wave a row.  The first blocks also count the rows that the mean is over, a slice each.
+template <typename T>
+__global__ __launch_bounds__(NT) void list_sums_kernel(Logits p, ListIn q, Sums u) {
+  __shared__ double red[NT / 64];
+  const int lane = threadIdx.x & 63;
+  for (unsigned r = blockIdx.x * (NT / 64) + (threadIdx.x >> 6); r < p.rows; r += gridDim.x * (NT / 64)) {
+    if (q.mask && !q.mask[r]) continue;
+    const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r);
+    const size_t first = (size_t)r * q.k;
+    float m = -INFINITY, vref = -INFINITY;
+    ListSum o{};
+    for (int k = lane; k < q.k; k += 64) {
+      const int j = entry_index(q, first + k, p.vocab);
+      if (j < 0) {
+        o.bad += j == -2;
+        continue;
+      }
+      m = fmaxf(m, (float)x[j]);
+      const float v = q.val[first + k];
+      vref = fmaxf(vref, v == v ? v : INFINITY);
+      o.used += 1;
+    }
+    m = wave_max(m);
+    vref = q.tail ? 0.f : wave_max(vref);
+    if (vref == -INFINITY) vref = 0.f;                          // no entry, or none with mass
+    const float ref = finite_ref(m);
+    const double it = q.tail ? 1.0 : 1.0 / p.tau;
+    for (int k = lane; k < q.k; k += 64) {
+      const int j = entry_index(q, first + k, p.vocab);
+      if (j < 0) continue;
+      const float f = (float)x[j], d = (f - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
+      const double lv = ((double)q.val[first + k] - (double)vref) * it, ev = exp(lv);
+      o.s += (double)e;
+      o.w += (double)(fmaxf(d, D_MIN) * e);
+      o.z += ev;
+      if (ev != 0) {
+        o.plogp += ev * lv;
+        o.px += ev * ((double)f - (double)ref) / p.tau;
+      }
+    }
+    o.m = m;
+    o.vref = vref;
+    o.s = wave_sum64(o.s);
+    o.w = wave_sum64(o.w);
+    o.z = wave_sum64(o.z);
+    o.plogp = wave_sum64(o.plogp);
+    o.px = wave_sum64(o.px);
+    o.used = wave_sum64(o.used);
+    o.bad = wave_sum64(o.bad);
+    o.mass = o.z;
+    if (!q.tail && o.z != 0) {                                  // p = exp(lv) / Z
+      o.plogp = o.plogp / o.z - log(o.z);
+      o.px /= o.z;
+      o.mass = o.z / o.z;                                       // 1, or NaN
+    }
+    if (lane == 0) q.sum[r] = o;
+  }
+  if ((int)blockIdx.x < u.blocks) {
+    double n = 0;
+    for (unsigned r = blockIdx.x * NT + threadIdx.x; r < p.rows; r += u.blocks * NT) n += !q.mask || q.mask[r];
+    n = block_sum64(n, red);
+    if (threadIdx.x == 0) {
+      u.counted[blockIdx.x] = n;
+      if (blockIdx.x == 0) *u.counter = 0;
+    }
+  }
+}
+
+// Bits of the listed elements of [lo, lo + n), shifted so that a 16-byte vector's elements start at a multiple of VEC;
+// returns whether this thread met an index that was set before.
+__device__ __forceinline__ bool mark(uint32_t* bits, const ListIn& q, unsigned r, int lo, int n, int shift, int t, int threads) {
+  bool twice = false;
+  for (int k = t; k < q.k; k += threads) {
+    const long long j = load_index(q.idx, q.idx64, (size_t)r * q.k + k) - lo;
+    if (j < 0 || j >= n) continue;
+    const unsigned at = (unsigned)j + shift, bit = 1u << (at & 31);
+    twice |= (atomicOr(bits + (at >> 5), bit) & bit) != 0;
+  }
+  return twice;
+}
+
+__device__ __forceinline__ bool marked(const uint32_t* bits, unsigned at) { return bits[at >> 5] >> (at & 31) & 1; }
+
+// The entries of a row's list that lie in [lo, lo + n), over the stream that wrote them as if they were off it.
+template <typename T>
+__device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, unsigned r, const f32x4& a, const f32x4& b, float scale, int lo,
+                                           int n, const T* x, T* out, int t, int threads) {
+  const float cv = q.tail ? (float)(1.0 / LN2) : p.c;
+  const size_t first = (size_t)r * q.k;
+  for (int k = t; k < q.k; k += threads) {
+    const long long j = load_index(q.idx, q.idx64, first + k) - lo;
+    if (j < 0 || j >= n) continue;
+    float pk = 0.f;
+    if (b[2] != 0.f) {                                          // an index twice in this row: its entries' sum, in order
+      for (int i = 0; i < q.k; ++i)
+        if (load_index(q.idx, q.idx64, first + i) - lo == j) pk += __builtin_amdgcn_exp2f((q.val[first + i] - b[0]) * cv);
+    } else {
+      pk = __builtin_amdgcn_exp2f((q.val[first + k] - b[0]) * cv);
+    }
+    const float e = __builtin_amdgcn_exp2f(((float)x[j] - a[2]) * p.c);
+    out[j] = (T)(scale * (a[3] * e - b[1] * pk));
+  }
+}
+
+// what a later entry of the same token added to the list's own sums (a whole wave calls it)
+template <typename T>
+__device__ __forceinline__ void take_back_repeats(const Logits& p, const ListIn& q, unsigned r, const T* x, ListSum& o) {
+  const size_t first = (size_t)r * q.k;
+  const float ref = finite_ref((float)o.m);
+  double s = 0, w = 0, n = 0;
+  for (int k = threadIdx.x & 63; k < q.k; k += 64) {
+    const int j = entry_index(q, first + k, p.vocab);
+    bool again = false;
+    for (int i = 0; j >= 0 && i < k && !again; ++i) again = entry_index(q, first + i, p.vocab) == j;
+    if (!again) continue;
+    const float d = ((float)x[j] - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
+    s += (double)e;
+    w += (double)(fmaxf(d, D_MIN) * e);
+    n += 1;
+  }
+  o.s -= wave_sum64(s);
+  o.w -= wave_sum64(w);
+  o.used -= wave_sum64(n);
+}
+
+// A row's loss (not yet times its weight) and coefficients, from the statistics off the list and the list's own sums.
+__device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, const Part& off, const ListSum& o, double weight, bool repeated,
+                                              f32x4& a, f32x4& b) {
+  const float m = fmaxf(off.m, (float)o.m), ref = finite_ref(m);
+  float s_off = off.s, w_off = off.w;
+  rebase(s_off, w_off, off.m, ref, p.c);
+  const float shift = ((float)o.m - ref) * p.c;                 // o.m = -inf: nothing listed has mass, o.s = 0
+  const double f = (double)__builtin_amdgcn_exp2f(shift);
+  const double eps = (double)p.c * LN2 * p.tau - 1.0;           // c = (1 + eps) log2(e) / tau
+  const double s = o.s * f + (double)s_off, w = f * (o.w + (double)fmaxf(shift, D_MIN) * o.s) + (double)w_off;
+  const double ln_s = s == 0 ? -INFINITY : log(s - eps * LN2 * w);
+  double loss = 0;
+  if (o.mass != 0) loss = s == 0 ? INFINITY : o.plogp - (o.px + o.mass * (((double)finite_ref((float)o.m) - (double)ref) / p.tau - ln_s));
+  const double rest = q.tail && o.used < (double)p.vocab ? (o.mass < 1 ? 1 - o.mass : o.mass >= 1 ? 0.0 : o.mass) : 0.0;
+  double to_rest = 0;
+  if (rest != 0) {
+    const double ln_off = off.s == 0.f ? -INFINITY : log((double)off.s - eps * LN2 * (double)off.w) + ((double)finite_ref(off.m) - (double)ref) / p.tau;
+    loss += off.s == 0.f ? INFINITY : rest * (log(rest) - (ln_off - ln_s));
+    if (off.s != 0.f) to_rest = rest / (double)off.s;
+  }
+  const double gr = q.scale * weight * p.tau, total = o.mass + rest;
+  const double on = s == 0 ? 0.0 : gr * total / s;
+  const double back = (double)__builtin_amdgcn_exp2f((finite_ref(off.m) - ref) * p.c);
+  a = f32x4{finite_ref(off.m), s == 0 || off.s == 0.f ? 0.f : (float)(on * back - gr * to_rest), ref, (float)on};
+  b = f32x4{(float)o.vref, s == 0 || o.mass == 0 ? 0.f : (float)(q.tail ? gr : gr / o.z), repeated ? 1.f : 0.f, s == 0 || total == 0 ? 0.f : 1.f};
+  if (o.bad != 0) {
+    loss = NAN;
+    a[1] = a[3] = NAN;
+    b[3] = 1.f;
+  }
+  return loss;
+}
+
+template <typename T, typename S>
+__global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, Sums u, int words, T* __restrict__ grad) {
+  constexpr int TPR = S::TPR, VEC = Type<T>::VEC;
+  extern __shared__ uint32_t all_bits[];
+  __shared__ Part red[TPR / 64];
+  __shared__ f32x4 told[2];
+  const int t = threadIdx.x % TPR;
+  uint32_t* bits = all_bits + (threadIdx.x / TPR) * words;
+  const unsigned r = blockIdx.x * S::ROWS + threadIdx.x / TPR;
+  const bool counts = r < p.rows && (!q.mask || q.mask[r]);
+  const T* x = reinterpret_cast<const T*>(p.x) + (counts ? row_offset(p, r) : 0);
+  Row<T, TPR, S::NCH> row;
+  row.load(x, counts ? p.vocab : 0, t);                         // on their way while the bitmap is made
+  const int shift = (VEC - row.head % VEC) % VEC;
+  for (int i = t; i < words; i += TPR) bits[i] = 0;
+  __syncthreads();
+  bool twice = counts && mark(bits, q, r, 0, p.vocab, shift, t, TPR);
+  if (TPR == 64) {
+    __syncthreads();
+    twice = __any(twice);
+  } else {
+    twice = __syncthreads_or(twice);
+  }
+#pragma unroll
+  for (int i = 0; i < S::NCH; ++i) {
+    const int at = t + i * TPR;
+    if (at >= row.nv) continue;
+    const unsigned bit = row.head + at * VEC + shift;
+    const uint32_t on = bits[bit >> 5] >> (bit & 31) & ((1u << VEC) - 1);
+    if (on) {
+      float f[VEC];
+      Type<T>::unpack(row.v[i], f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
+      row.v[i] = Type<T>::pack(f);
+    }
+  }
+  if (row.extra_at >= 0 && marked(bits, row.extra_at + shift)) row.extra = -INFINITY;
+  Part m = row.stats(p.c);
+  for (int i = t + S::NCH * TPR; i < row.nv; i += TPR) {
+    float f[VEC];
+    Type<T>::unpack(row.body()[i], f);
+    const unsigned bit = row.head + i * VEC + shift;
+    const uint32_t on = bits[bit >> 5] >> (bit & 31) & ((1u << VEC) - 1);
+    if (on)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
+    take<VEC>(m, f, p.c);
+  }
+  m = row_join<TPR>(m, p.c, red);
+  f32x4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
+  if ((TPR == 64 || threadIdx.x < 64) && r < p.rows) {
+    float loss = 0.f;
+    if (counts) {
+      const double w = one_over_counted(u);
+      ListSum o = q.sum[r];
+      if (twice) take_back_repeats(p, q, r, x, o);
+      loss = (float)(w * p.tau * p.tau * finish_list(p, q, m, o, w, twice, a, b));
+    }
+    if (t == 0) {
+      u.terms[r] = f32x4{loss, 0.f, 0.f, 0.f};
+      if (q.row) {
+        q.row[2 * (size_t)r] = a;
+        q.row[2 * (size_t)r + 1] = b;
+      }
+      if (TPR > 64) {
+        told[0] = a;
+        told[1] = b;
+      }
+    }
+  }
+  if (!grad) return;
+  if (TPR > 64) {
+    __syncthreads();
+    a = told[0];
+    b = told[1];
+  }
+  T* out = grad + (size_t)r * p.vocab;
+  const bool zero = b[3] == 0.f;
+  if (r < p.rows) {
+    if (zero) store_zeros<T, TPR>(out, p.vocab, t);
+    else row.store(out, f32x4{a[0], a[1], 0.f, 0.f}, p.c, -1);
+  }
+  __syncthreads();                                              // a listed element is written twice, in this order
+  if (!zero) patch_list<T>(p, q, r, a, b, 1.f, 0, p.vocab, x, out, t, TPR);
+}
+
+// the gradient again, for another upstream gradient or a second time
+template <typename T, int TPR>
+__global__ __launch_bounds__(NT) void list_grad_kernel(Logits p, ListIn q, const float* gout, int skip_if_one, int splits, int chunk,
+                                                       T* __restrict__ grad) {
+  constexpr int VEC = Type<T>::VEC;
+  const float scale = gout ? gout[0] : 1.f;
+  if (skip_if_one && scale == 1.f) return;
+  const int t = threadIdx.x % TPR;
+  const unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const unsigned r = (unsigned)(part / splits);
+  const bool live = r < p.rows;
+  const int lo = live ? std::min((long long)(part % splits) * chunk, (long long)p.vocab) : 0;
+  const int n = live ? std::min((long long)chunk, (long long)p.vocab - lo) : 0;
+  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+  const f32x4 a = live ? q.row[2 * (size_t)r] : zero4, b = live ? q.row[2 * (size_t)r + 1] : zero4;
+  const bool zero = b[3] == 0.f;
+  T* out = grad + (live ? (size_t)r * p.vocab + lo : 0);
+  const T* x = reinterpret_cast<const T*>(p.x) + (live ? row_offset(p, r) + lo : 0);
+  if (zero) {
+    store_zeros<T, TPR>(out, n, t);
+  } else {
+    const f32x4 k = {a[0], a[1] * scale, 0.f, 0.f};
+    const int head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+    const int nv = (n - head) / VEC, behind = head + nv * VEC;
+    const u32x4* v = reinterpret_cast<const u32x4*>(x + head);
+    u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
+    for (int i = t; i < nv; i += TPR) o[i] = gradient_vector<T, false>(v[i], k, p.c, -1);
+    if (t < head) out[t] = gradient_one<T, false>((float)x[t], k, p.c, false);
+    if (t < n - behind) out[behind + t] = gradient_one<T, false>((float)x[behind + t], k, p.c, false);
+  }
+  __syncthreads();                                              // a listed element is written twice, in this order
+  if (!zero) patch_list<T>(p, q, r, a, b, scale, lo, n, x, out, t, TPR);
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------
+template <typename T>
+int launch_list_grad_t(const char* who, const Logits& p, const ListIn& q, const float* gout, int skip, void* grad, hipStream_t s) {
+  const long long bytes = (long long)p.vocab * (long long)sizeof(T);
+  const int tpr = bytes <= 4096 ? 64 : NT;
+  const int chunk = bytes <= 4096 ? p.vocab : 16384 / (int)sizeof(T);
+  const int splits = (int)st::cdivll(p.vocab, chunk);
+  const long long blocks = st::cdivll((long long)p.rows * splits, NT / tpr);
+  if (blocks > 0x7fffffffLL) return st::fail(ST_ERR_BAD_ARG, "%s: too many rows", who);
+  if (tpr == 64) hipLaunchKernelGGL((list_grad_kernel<T, 64>), dim3((unsigned)blocks), dim3(NT), 0, s, p, q, gout, skip, splits, chunk, (T*)grad);
+  else hipLaunchKernelGGL((list_grad_kernel<T, NT>), dim3((unsigned)blocks), dim3(NT), 0, s, p, q, gout, skip, splits, chunk, (T*)grad);
+  return st::check_launch(who);
+}
+
+}  // namespace
+
+extern "C" size_t st_distill_workspace_bytes(long long rows) {
+  if (rows <= 0 || rows > 0x7fffffffLL) return 0;
+  return sums_bytes(rows) + align256((size_t)rows * sizeof(ListSum));
+}
+
+extern "C" int st_distill_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer, long long s_inner, int vocab,
+                                   const void* teacher_idx, int idx64, const float* teacher_val, int k, const unsigned char* mask, double tau,
+                                   int tail, double scale, float* loss, float* row_grad, void* grad, void* workspace, st_stream_t stream) {
+  const char* who = "st_distill_loss_fwd";
+  Logits p = make_logits(x, rows, inner, s_outer, s_inner, vocab, nullptr, 0, 0, tau);
+  int rc;
+  if (bad_logits(who, p, dtype, rows, inner, s_outer, s_inner, &rc)) return rc;
+  ST_REQUIRE(rows > 0 && k > 0, "%s: rows=%lld k=%d", who, rows, k);
+  ST_REQUIRE(vocab <= MAX_VOCAB, "%s: vocab=%d (at most %d)", who, vocab, MAX_VOCAB);
+  ST_REQUIRE(teacher_idx && teacher_val && loss && workspace, "%s: null pointer", who);
+  hipStream_t s = (hipStream_t)stream;
+  Space w{reinterpret_cast<char*>(workspace)};
+  Sums u = make_sums(w, rows, loss, nullptr, scale, 0.0, 0.0);
+  ListIn q{};
+  q.idx = teacher_idx;
+  q.idx64 = idx64;
+  q.val = teacher_val;
+  q.k = k;
+  q.mask = mask;
+  q.tail = tail;
+  q.scale = scale;
+  q.sum = w.take<ListSum>((size_t)rows);
+  q.row = reinterpret_cast<f32x4*>(row_grad);
+  const unsigned blocks = (unsigned)std::min<long long>(2048, st::cdivll(rows, NT / 64));
+  u.blocks = (int)std::min<long long>(std::min<unsigned>(COUNT_BLOCKS, blocks), st::cdivll(rows, 1024));
+  return with_type(dtype, [&](auto type) {
+    using T = decltype(type);
+    hipLaunchKernelGGL(list_sums_kernel<T>, dim3(blocks), dim3(NT), 0, s, p, q, u);
+    const int words = (vocab + Type<T>::VEC + 31) / 32;
+    const int launched = with_shape((long long)vocab * (long long)sizeof(T), [&](auto shape) -> int {
+      using S = decltype(shape);
+      const size_t lds = (size_t)words * 4 * S::ROWS;
+      if (lds > MAX_PLAIN_LDS) {                                // the attribute is set once a device: to the most that any call needs
+        static st::DynLdsOptIn opt_in;
+        const int rc = st::allow_dynamic_lds(distill_kernel<T, S>, (size_t)(MAX_VOCAB / 8 + 64), opt_in, who);
+        if (rc != ST_OK) return rc;
+      }
+      hipLaunchKernelGGL((distill_kernel<T, S>), dim3((unsigned)st::cdivll(rows, S::ROWS)), dim3(S::BLOCK), lds, s, p, q, u, words, (T*)grad);
+      return ST_OK;
+    });
+    if (launched != ST_OK) return launched;
+    launch_sum_terms(u, s);
+    return st::check_launch(who);
+  });
+}
+
+extern "C" int st_distill_loss_bwd(const void* x, int dtype, long long rows, long long inner, long long s_outer, long long s_inner, int vocab,
+                                   const void* teacher_idx, int idx64, const float* teacher_val, int k, double tau, int tail,
+                                   const float* row_grad, const float* gout, int grad_is_for_one, void* grad, st_stream_t stream) {
+  const char* who = "st_distill_loss_bwd";
+  Logits p = make_logits(x, rows, inner, s_outer, s_inner, vocab, nullptr, 0, 0, tau);
+  int rc;
+  if (bad_logits(who, p, dtype, rows, inner, s_outer, s_inner, &rc)) return rc;
+  if (rows == 0) return ST_OK;
+  ST_REQUIRE(teacher_idx && teacher_val && row_grad && grad && k > 0, "%s: null pointer", who);
+  ListIn q{};
+  q.idx = teacher_idx;
+  q.idx64 = idx64;
+  q.val = teacher_val;
+  q.k = k;
+  q.tail = tail;
+  q.row = const_cast<f32x4*>(reinterpret_cast<const f32x4*>(row_grad));
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == ST_F32) return launch_list_grad_t<float>(who, p, q, gout, grad_is_for_one, grad, s);
+  if (dtype == ST_BF16) return launch_list_grad_t<__bf16>(who, p, q, gout, grad_is_for_one, grad, s);
+  return launch_list_grad_t<_Float16>(who, p, q, gout, grad_is_for_one, grad, s);
+}

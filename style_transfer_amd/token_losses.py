@@ -16,6 +16,9 @@ What they have in common:
 * With nothing that counts a loss is 0.  ``scale`` multiplies a loss and its gradient (a weight, 1 / accumulation steps, a
   static loss scale).
 * Results do not depend on the run: every sum has a fixed order.
+* ``clipped_policy_loss`` and ``topk_distill_loss`` write the gradient of logits that require one in the forward pass, while
+  a row is on chip.  A backward pass with an upstream gradient of 1 hands it over; another one (a loss weight outside, a
+  dynamic loss scale) computes it again from the logits: pass a known factor as ``scale``.
 """
 from __future__ import annotations
 
@@ -176,7 +179,7 @@ class _TokenLogProbsFunction(torch.autograd.Function):
             return None, None, None, None, None
         x, labels, state = ctx.saved_tensors
         lib = _lib.load()
-        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        grad = _grad_buffer(x)
         g_logp = None if g_logp is None else _gout(g_logp)
         g_entropy = None if g_entropy is None else _gout(g_entropy)
         with _on(x):
@@ -200,13 +203,24 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
 
 
 # ---- the two losses whose rows go through the label's log-probability -------------------------------------------------------------
+def _grad_buffer(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _take_grad(ctx, x):
+    """(buffer, 1) the first time: it holds the gradient for an upstream gradient of 1, written by the forward kernel while the
+    rows were on chip.  The buffer is given away, so a second backward pass gets a new one, (buffer, 0)."""
+    grad, ctx.grad = getattr(ctx, "grad", None), None
+    return (_grad_buffer(x), 0) if grad is None else (grad, 1)
+
+
 def _token_loss_bwd(ctx, x, labels, row_grad, gout):
     lib = _lib.load()
-    grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    grad, for_one = _take_grad(ctx, x)
     gout = _gout(gout)
     with _on(x):
         _lib.check(lib.st_token_loss_bwd(*_logits_args(x), *_label_args(labels, ctx.ignore), ctx.tau, row_grad.data_ptr(), gout.data_ptr(),
-                                         grad.data_ptr(), _lib.stream_ptr()), "st_token_loss_bwd")
+                                         for_one, grad.data_ptr(), _lib.stream_ptr()), "st_token_loss_bwd")
     return grad
 
 
@@ -288,14 +302,15 @@ class _PolicyFunction(torch.autograd.Function):
         rows, need = args[2], ctx.needs_input_grad[0]
         loss, stats = _f32(x), _f32(x, 4)
         row_grad = _f32(x, rows, 4) if need else None
+        grad = _grad_buffer(x) if need else None
         with _on(x):
             work = _buffer(x, lib.st_token_workspace_bytes(args[1], rows, args[6], sequences))
             _lib.check(lib.st_policy_loss_fwd(*args, *_label_args(labels, ignore), tau, _ptr(cu), sequences, old.data_ptr(), adv.data_ptr(),
                                               int(adv.shape != labels.shape), _ptr(ref), low, high, kl, ent, per_sequence, scale,
-                                              loss.data_ptr(), stats.data_ptr(), _ptr(row_grad), work.data_ptr(), _lib.stream_ptr()),
-                       "st_policy_loss_fwd")
+                                              loss.data_ptr(), stats.data_ptr(), _ptr(row_grad), _ptr(grad), work.data_ptr(),
+                                              _lib.stream_ptr()), "st_policy_loss_fwd")
         ctx.mark_non_differentiable(stats)
-        ctx.tau, ctx.ignore = tau, ignore
+        ctx.tau, ctx.ignore, ctx.grad = tau, ignore, grad
         if need:
             ctx.save_for_backward(x, labels, row_grad)
         return loss, stats
@@ -352,12 +367,13 @@ class _DistillFunction(torch.autograd.Function):
         rows, need = args[2], ctx.needs_input_grad[0]
         loss = _f32(x)
         row_grad = _f32(x, rows, 8) if need else None
+        grad = _grad_buffer(x) if need else None
         entries = (idx.data_ptr(), int(idx.dtype == torch.int64), val.data_ptr(), idx.shape[-1])
         with _on(x):
-            work = _buffer(x, lib.st_distill_workspace_bytes(args[1], rows, args[6]))
-            _lib.check(lib.st_distill_loss_fwd(*args, *entries, _ptr(mask), tau, tail, scale, loss.data_ptr(), _ptr(row_grad), work.data_ptr(),
-                                               _lib.stream_ptr()), "st_distill_loss_fwd")
-        ctx.tau, ctx.tail = tau, tail
+            work = _buffer(x, lib.st_distill_workspace_bytes(rows))
+            _lib.check(lib.st_distill_loss_fwd(*args, *entries, _ptr(mask), tau, tail, scale, loss.data_ptr(), _ptr(row_grad), _ptr(grad),
+                                               work.data_ptr(), _lib.stream_ptr()), "st_distill_loss_fwd")
+        ctx.tau, ctx.tail, ctx.grad = tau, tail, grad
         if need:
             ctx.save_for_backward(x, idx, val, row_grad)
         return loss
@@ -367,11 +383,11 @@ class _DistillFunction(torch.autograd.Function):
     def backward(ctx, gout):
         x, idx, val, row_grad = ctx.saved_tensors
         lib = _lib.load()
-        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        grad, for_one = _take_grad(ctx, x)
         gout = _gout(gout)
         with _on(x):
             _lib.check(lib.st_distill_loss_bwd(*_logits_args(x), idx.data_ptr(), int(idx.dtype == torch.int64), val.data_ptr(), idx.shape[-1],
-                                               ctx.tau, ctx.tail, row_grad.data_ptr(), gout.data_ptr(), grad.data_ptr(),
+                                               ctx.tau, ctx.tail, row_grad.data_ptr(), gout.data_ptr(), for_one, grad.data_ptr(),
                                                _lib.stream_ptr()), "st_distill_loss_bwd")
         return grad, None, None, None, None, None, None
 
@@ -388,7 +404,7 @@ def topk_distill_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     they are the teacher's log-probabilities (at ``temperature``, over its whole vocabulary), and all tokens that are not listed
     form one more entry of the sum, with ``1 - sum_k p_k`` and the student's probability of the same tokens.
 
-    A position with no used entry contributes 0.  An index of ``V`` or more makes its position's loss and gradient NaN."""
+    At most 2^20 tokens.  A position with no used entry contributes 0.  An index of ``V`` or more makes its position's loss and gradient NaN."""
     _logits_args(logits)
     shape = logits.shape[:-1]
     if not isinstance(teacher_indices, torch.Tensor) or teacher_indices.dim() != logits.dim() or teacher_indices.shape[-1] == 0:

@@ -89,16 +89,17 @@ def test_c_entries_return_errors():
                   (p + 2, 0, 4, 4, 0, 10, 10), (p, 0, 2 ** 31, 4, 0, 10, 10)):
         assert lib.st_token_logprobs_fwd(*wrong, *labels, 1.0, p, None, None, p, None) == -1, wrong
         assert lib.st_token_logprobs_bwd(*wrong, *labels, 1.0, p, p, None, p, None) == -1, wrong
-        assert lib.st_token_loss_bwd(*wrong, *labels, 1.0, p, None, p, None) == -1, wrong
-        assert lib.st_distill_loss_bwd(*wrong, p, 1, p, 3, 1.0, 0, p, None, p, None) == -1, wrong
+        assert lib.st_token_loss_bwd(*wrong, *labels, 1.0, p, None, 0, p, None) == -1, wrong
+        assert lib.st_distill_loss_bwd(*wrong, p, 1, p, 3, 1.0, 0, p, None, 0, p, None) == -1, wrong
     for tau in (0.0, -1.0, math.inf, math.nan, 1e-60):
         assert lib.st_token_logprobs_fwd(*good, *labels, tau, p, None, None, p, None) == -1
     pref = lambda pairs, kind, beta, eps: lib.st_preference_loss_fwd(*good, *labels, None, pairs, None, kind, 0, beta, eps, 1.0, p, p, None, p, None)  # noqa: E731
     assert pref(1, 0, 0.1, 0.0) == -1                          # 4 rows of 4 are one sequence, not two
     assert pref(0, 0, 0.1, 0.0) == -1
-    policy = lambda seqs, low: lib.st_policy_loss_fwd(*good, *labels, 1.0, None, seqs, p, p, 0, None, low, 0.2, 0.0, 0.0, 0, 1.0, p, p, None, p, None)  # noqa: E731
+    policy = lambda seqs, low: lib.st_policy_loss_fwd(*good, *labels, 1.0, None, seqs, p, p, 0, None, low, 0.2, 0.0, 0.0, 0, 1.0, p, p, None, None, p, None)  # noqa: E731
     assert policy(2, 0.2) == -1 and policy(1, 1.5) == -1
-    assert lib.st_distill_loss_fwd(*good, p, 1, p, 0, None, 1.0, 0, 1.0, p, None, p, None) == -1
+    assert lib.st_distill_loss_fwd(*good, p, 1, p, 0, None, 1.0, 0, 1.0, p, None, None, p, None) == -1
+    assert lib.st_distill_loss_fwd(p, 0, 4, 4, 0, 2 ** 21, 2 ** 21, p, 1, p, 3, None, 1.0, 0, 1.0, p, None, None, p, None) == -1
     assert lib.st_token_workspace_bytes(0, -1, 10, 0) == 0 and lib.st_token_workspace_bytes(1, 1, 131072, 2) > 0
 
 
