@@ -7,9 +7,10 @@
 // q_rest comes from its own sum over the elements off the list (a bitmap in LDS tells them apart): 1 - sum q_k would keep
 // no digit of it where the student is sure of a listed token.  Entries that name the same token add up.
 //
-// A first kernel takes what the lists alone say (a wave a row, in fp64, K values and K gathered logits); the second holds a
-// row in registers, with -inf in place of the listed elements, so that its statistics are those off the list, and writes
-// the gradient in two steps: the stream as if nothing were listed, then the K entries over it.
+// One kernel holds a row in registers, with -inf in place of the listed elements, so that its statistics are those off the
+// list, and writes the gradient in two steps: the stream as if nothing were listed, then the K entries over it.  What the
+// list says by itself (K values, K gathered logits) is its first wave's work before that wave asks for its share of the row:
+// the other waves' share is on its way meanwhile, and the list needs none of the registers that the row will.
 #include "token_rows.h"
 
 namespace {
@@ -21,11 +22,11 @@ constexpr size_t MAX_PLAIN_LDS = 48 << 10;   // dynamic LDS that a kernel gets w
 
 // what the list of a row says by itself
 struct ListSum {
-  double m, s, w;            // the listed logits' maximum, and S and W of the listed tokens seen from it (once each entry)
-  double vref, z;            // the values' maximum and sum of exp((v - vref) / tau); tail: 0 and unused
-  double mass, plogp, px;    // P, sum p ln p, sum p (x - m) / tau
-  double used;               // entries
-  double bad;                // an index outside the vocabulary
+  float m, s, w;             // the listed logits' maximum, S and W of the listed tokens seen from it (once each entry)
+  float vref;                // the values' maximum; tail: 0
+  double z;                  // sum of exp((v - vref) / tau); tail: the mass itself
+  double gap;                // sum of exp((v - vref) / tau) ((v - vref) / tau - (x - m) / tau)
+  int used, bad;             // entries; any outside the vocabulary
 };
 
 struct ListIn {
@@ -36,15 +37,8 @@ struct ListIn {
   const unsigned char* mask; // [rows] or null
   int tail;
   double scale;
-  ListSum* sum;              // [rows]
   f32x4* row;                // [rows][2]: (m_off, alpha_off, m, alpha_on), (vref, g / Z, an index twice, not zero) or null
 };
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
-}
 
 // index of entry k: -1 unused, -2 outside the vocabulary
 __device__ __forceinline__ int entry_index(const ListIn& q, size_t at, int vocab) {
@@ -52,72 +46,57 @@ __device__ __forceinline__ int entry_index(const ListIn& q, size_t at, int vocab
   return j < 0 ? -1 : j >= vocab ? -2 : (int)j;
 }
 
-// A wave a row.  The first blocks also count the rows that the mean is over, a slice each.
+// a whole wave calls it
 template <typename T>
-__global__ __launch_bounds__(NT) void list_sums_kernel(Logits p, ListIn q, Sums u) {
-  __shared__ double red[NT / 64];
+__device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, unsigned r, const T* x) {
   const int lane = threadIdx.x & 63;
-  for (unsigned r = blockIdx.x * (NT / 64) + (threadIdx.x >> 6); r < p.rows; r += gridDim.x * (NT / 64)) {
-    if (q.mask && !q.mask[r]) continue;
-    const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r);
-    const size_t first = (size_t)r * q.k;
-    float m = -INFINITY, vref = -INFINITY;
-    ListSum o{};
-    for (int k = lane; k < q.k; k += 64) {
-      const int j = entry_index(q, first + k, p.vocab);
-      if (j < 0) {
-        o.bad += j == -2;
-        continue;
-      }
-      m = fmaxf(m, (float)x[j]);
-      const float v = q.val[first + k];
-      vref = fmaxf(vref, v == v ? v : INFINITY);
-      o.used += 1;
-    }
-    m = wave_max(m);
-    vref = q.tail ? 0.f : wave_max(vref);
-    if (vref == -INFINITY) vref = 0.f;                          // no entry, or none with mass
-    const float ref = finite_ref(m);
-    const double it = q.tail ? 1.0 : 1.0 / p.tau;
-    for (int k = lane; k < q.k; k += 64) {
-      const int j = entry_index(q, first + k, p.vocab);
-      if (j < 0) continue;
-      const float f = (float)x[j], d = (f - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
-      const double lv = ((double)q.val[first + k] - (double)vref) * it, ev = exp(lv);
-      o.s += (double)e;
-      o.w += (double)(fmaxf(d, D_MIN) * e);
-      o.z += ev;
-      if (ev != 0) {
-        o.plogp += ev * lv;
-        o.px += ev * ((double)f - (double)ref) / p.tau;
-      }
-    }
-    o.m = m;
-    o.vref = vref;
-    o.s = wave_sum64(o.s);
-    o.w = wave_sum64(o.w);
-    o.z = wave_sum64(o.z);
-    o.plogp = wave_sum64(o.plogp);
-    o.px = wave_sum64(o.px);
-    o.used = wave_sum64(o.used);
-    o.bad = wave_sum64(o.bad);
-    o.mass = o.z;
-    if (!q.tail && o.z != 0) {                                  // p = exp(lv) / Z
-      o.plogp = o.plogp / o.z - log(o.z);
-      o.px /= o.z;
-      o.mass = o.z / o.z;                                       // 1, or NaN
-    }
-    if (lane == 0) q.sum[r] = o;
+  const size_t first = (size_t)r * q.k;
+  ListSum o;
+  float m = -INFINITY, vref = -INFINITY;
+  int used = 0, bad = 0;
+  for (int k = lane; k < q.k; k += 64) {
+    const int j = entry_index(q, first + k, p.vocab);
+    const float v = q.val[first + k];
+    bad |= j == -2;
+    if (j < 0) continue;
+    m = fmaxf(m, (float)x[j]);
+    vref = fmaxf(vref, v == v ? v : INFINITY);
+    ++used;
   }
-  if ((int)blockIdx.x < u.blocks) {
-    double n = 0;
-    for (unsigned r = blockIdx.x * NT + threadIdx.x; r < p.rows; r += u.blocks * NT) n += !q.mask || q.mask[r];
-    n = block_sum64(n, red);
-    if (threadIdx.x == 0) {
-      u.counted[blockIdx.x] = n;
-      if (blockIdx.x == 0) *u.counter = 0;
-    }
+  o.m = lanes_max(m);
+  o.vref = q.tail ? 0.f : lanes_max(vref);
+  if (o.vref == -INFINITY) o.vref = 0.f;                        // no entry, or none with mass
+  o.used = (int)lanes_sum((float)used);
+  o.bad = __any(bad);
+  const float ref = finite_ref(o.m);
+  const double it = q.tail ? 1.0 : p.inv_tau;
+  float s = 0.f, w = 0.f;
+  double z = 0.0, gap = 0.0;
+  for (int k = lane; k < q.k; k += 64) {
+    const int j = entry_index(q, first + k, p.vocab);
+    if (j < 0) continue;
+    const float f = (float)x[j], d = (f - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
+    const double lv = ((double)q.val[first + k] - (double)o.vref) * it;
+    const float ev = exp_wide(lv);
+    s += e;
+    w = fmaf(fmaxf(d, D_MIN), e, w);
+    z += (double)ev;
+    if (ev != 0.f) gap += (double)ev * (lv - ((double)f - (double)ref) * p.inv_tau);
   }
+  o.s = lanes_sum(s);
+  o.w = lanes_sum(w);
+  o.z = lanes_sum(z);
+  o.gap = lanes_sum(gap);
+  return o;
+}
+
+// the rows that the mean is over
+__global__ __launch_bounds__(1024) void count_mask_kernel(const unsigned char* mask, Sums u) {
+  __shared__ double red[16];
+  double n = 0;
+  for (unsigned r = blockIdx.x * 1024 + threadIdx.x; r < u.rows; r += u.blocks * 1024) n += mask[r] != 0;
+  n = block_sum64(n, red);
+  if (threadIdx.x == 0) u.counted[blockIdx.x] = n;
 }
 
 // Bits of the listed elements of [lo, lo + n), shifted so that a 16-byte vector's elements start at a multiple of VEC;
@@ -156,53 +135,57 @@ __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, uns
   }
 }
 
-// what a later entry of the same token added to the list's own sums (a whole wave calls it)
+// the list's own sums without what later entries of a token added to the student's side (a whole wave calls it)
 template <typename T>
-__device__ __forceinline__ void take_back_repeats(const Logits& p, const ListIn& q, unsigned r, const T* x, ListSum& o) {
+__device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn& q, unsigned r, const T* x, ListSum o) {
   const size_t first = (size_t)r * q.k;
-  const float ref = finite_ref((float)o.m);
-  double s = 0, w = 0, n = 0;
+  const float ref = finite_ref(o.m);
+  float s = 0, w = 0, n = 0;
   for (int k = threadIdx.x & 63; k < q.k; k += 64) {
     const int j = entry_index(q, first + k, p.vocab);
     bool again = false;
     for (int i = 0; j >= 0 && i < k && !again; ++i) again = entry_index(q, first + i, p.vocab) == j;
-    if (!again) continue;
-    const float d = ((float)x[j] - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
-    s += (double)e;
-    w += (double)(fmaxf(d, D_MIN) * e);
-    n += 1;
+    if (again) {
+      n += 1;
+    } else if (j >= 0) {
+      const float d = ((float)x[j] - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
+      s += e;
+      w = fmaf(fmaxf(d, D_MIN), e, w);
+    }
   }
-  o.s -= wave_sum64(s);
-  o.w -= wave_sum64(w);
-  o.used -= wave_sum64(n);
+  o.s = lanes_sum(s);
+  o.w = lanes_sum(w);
+  o.used -= (int)lanes_sum(n);
+  return o;
 }
 
 // A row's loss (not yet times its weight) and coefficients, from the statistics off the list and the list's own sums.
 __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, const Part& off, const ListSum& o, double weight, bool repeated,
                                               f32x4& a, f32x4& b) {
-  const float m = fmaxf(off.m, (float)o.m), ref = finite_ref(m);
-  float s_off = off.s, w_off = off.w;
+  const float ref = finite_ref(fmaxf(off.m, o.m)), ref_off = finite_ref(off.m), ref_list = finite_ref(o.m);
+  float s_off = off.s, w_off = off.w, s_list = o.s, w_list = o.w;
   rebase(s_off, w_off, off.m, ref, p.c);
-  const float shift = ((float)o.m - ref) * p.c;                 // o.m = -inf: nothing listed has mass, o.s = 0
-  const double f = (double)__builtin_amdgcn_exp2f(shift);
-  const double eps = (double)p.c * LN2 * p.tau - 1.0;           // c = (1 + eps) log2(e) / tau
-  const double s = o.s * f + (double)s_off, w = f * (o.w + (double)fmaxf(shift, D_MIN) * o.s) + (double)w_off;
-  const double ln_s = s == 0 ? -INFINITY : log(s - eps * LN2 * w);
+  rebase(s_list, w_list, o.m, ref, p.c);
+  const float s = s_list + s_off, w = w_list + w_off;
+  const double ln_s = ln_wide(fmaf(-p.eps_ln2, w, s));
+  const double mass = q.tail ? o.z : o.z == 0 ? 0.0 : o.z / o.z;                       // 1, or NaN
   double loss = 0;
-  if (o.mass != 0) loss = s == 0 ? INFINITY : o.plogp - (o.px + o.mass * (((double)finite_ref((float)o.m) - (double)ref) / p.tau - ln_s));
-  const double rest = q.tail && o.used < (double)p.vocab ? (o.mass < 1 ? 1 - o.mass : o.mass >= 1 ? 0.0 : o.mass) : 0.0;
-  double to_rest = 0;
-  if (rest != 0) {
-    const double ln_off = off.s == 0.f ? -INFINITY : log((double)off.s - eps * LN2 * (double)off.w) + ((double)finite_ref(off.m) - (double)ref) / p.tau;
-    loss += off.s == 0.f ? INFINITY : rest * (log(rest) - (ln_off - ln_s));
-    if (off.s != 0.f) to_rest = rest / (double)off.s;
+  if (mass != 0) {
+    loss = (q.tail ? o.gap : o.gap / o.z - (double)ln_wide((float)o.z)) + mass * (ln_s - ((double)ref_list - (double)ref) * p.inv_tau);
+    if (s == 0.f) loss = INFINITY;
   }
-  const double gr = q.scale * weight * p.tau, total = o.mass + rest;
-  const double on = s == 0 ? 0.0 : gr * total / s;
-  const double back = (double)__builtin_amdgcn_exp2f((finite_ref(off.m) - ref) * p.c);
-  a = f32x4{finite_ref(off.m), s == 0 || off.s == 0.f ? 0.f : (float)(on * back - gr * to_rest), ref, (float)on};
-  b = f32x4{(float)o.vref, s == 0 || o.mass == 0 ? 0.f : (float)(q.tail ? gr : gr / o.z), repeated ? 1.f : 0.f, s == 0 || total == 0 ? 0.f : 1.f};
-  if (o.bad != 0) {
+  const double rest = q.tail && o.used < p.vocab ? (mass < 1 ? 1 - mass : mass >= 1 ? 0.0 : mass) : 0.0;
+  const float inv = reciprocal(s), inv_off = reciprocal(off.s);
+  if (rest != 0) {
+    const double ln_off = ln_wide(fmaf(-p.eps_ln2, off.w, off.s)) + ((double)ref_off - (double)ref) * p.inv_tau;
+    loss += off.s == 0.f ? INFINITY : rest * (ln_wide((float)rest) - (ln_off - ln_s));
+  }
+  const double gr = q.scale * weight * p.tau, total = mass + rest;
+  const float on = s == 0.f ? 0.f : (float)(gr * total * (double)inv);
+  const double back = (double)__builtin_amdgcn_exp2f((ref_off - ref) * p.c);
+  a = f32x4{ref_off, s == 0.f || off.s == 0.f ? 0.f : (float)(gr * (total * (double)inv * back - rest * (double)inv_off)), ref, on};
+  b = f32x4{o.vref, s == 0.f || mass == 0 ? 0.f : (float)(q.tail ? gr : gr / o.z), repeated ? 1.f : 0.f, s == 0.f || total == 0 ? 0.f : 1.f};
+  if (o.bad) {
     loss = NAN;
     a[1] = a[3] = NAN;
     b[3] = 1.f;
@@ -221,8 +204,11 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   const unsigned r = blockIdx.x * S::ROWS + threadIdx.x / TPR;
   const bool counts = r < p.rows && (!q.mask || q.mask[r]);
   const T* x = reinterpret_cast<const T*>(p.x) + (counts ? row_offset(p, r) : 0);
+  ListSum list{};
+  if (counts && (TPR == 64 || threadIdx.x < 64)) list = sum_list(p, q, r, x);
   Row<T, TPR, S::NCH> row;
   row.load(x, counts ? p.vocab : 0, t);                         // on their way while the bitmap is made
+  const double share = q.mask ? counted_share(u) : 0.0;
   const int shift = (VEC - row.head % VEC) % VEC;
   for (int i = t; i < words; i += TPR) bits[i] = 0;
   __syncthreads();
@@ -264,10 +250,9 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   if ((TPR == 64 || threadIdx.x < 64) && r < p.rows) {
     float loss = 0.f;
     if (counts) {
-      const double w = one_over_counted(u);
-      ListSum o = q.sum[r];
-      if (twice) take_back_repeats(p, q, r, x, o);
-      loss = (float)(w * p.tau * p.tau * finish_list(p, q, m, o, w, twice, a, b));
+      const double w = q.mask ? one_over(share) : 1.0 / u.rows;
+      if (twice) list = without_repeats(p, q, r, x, list);
+      loss = (float)(w * p.tau * p.tau * finish_list(p, q, m, list, w, twice, a, b));
     }
     if (t == 0) {
       u.terms[r] = f32x4{loss, 0.f, 0.f, 0.f};
@@ -305,30 +290,33 @@ __global__ __launch_bounds__(NT) void list_grad_kernel(Logits p, ListIn q, const
   const float scale = gout ? gout[0] : 1.f;
   if (skip_if_one && scale == 1.f) return;
   const int t = threadIdx.x % TPR;
-  const unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
-  const unsigned r = (unsigned)(part / splits);
-  const bool live = r < p.rows;
-  const int lo = live ? std::min((long long)(part % splits) * chunk, (long long)p.vocab) : 0;
-  const int n = live ? std::min((long long)chunk, (long long)p.vocab - lo) : 0;
-  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
-  const f32x4 a = live ? q.row[2 * (size_t)r] : zero4, b = live ? q.row[2 * (size_t)r + 1] : zero4;
-  const bool zero = b[3] == 0.f;
-  T* out = grad + (live ? (size_t)r * p.vocab + lo : 0);
-  const T* x = reinterpret_cast<const T*>(p.x) + (live ? row_offset(p, r) + lo : 0);
-  if (zero) {
-    store_zeros<T, TPR>(out, n, t);
-  } else {
-    const f32x4 k = {a[0], a[1] * scale, 0.f, 0.f};
-    const int head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-    const int nv = (n - head) / VEC, behind = head + nv * VEC;
-    const u32x4* v = reinterpret_cast<const u32x4*>(x + head);
-    u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
-    for (int i = t; i < nv; i += TPR) o[i] = gradient_vector<T, false>(v[i], k, p.c, -1);
-    if (t < head) out[t] = gradient_one<T, false>((float)x[t], k, p.c, false);
-    if (t < n - behind) out[behind + t] = gradient_one<T, false>((float)x[behind + t], k, p.c, false);
+  const unsigned long long parts = (unsigned long long)p.rows * splits, step = (unsigned long long)gridDim.x * (NT / TPR);
+  for (unsigned long long first = (unsigned long long)blockIdx.x * (NT / TPR); first < parts; first += step) {     // the same for a block's threads
+    const unsigned long long part = first + threadIdx.x / TPR;
+    const unsigned r = (unsigned)(part / splits);
+    const bool live = part < parts;
+    const int lo = live ? std::min((long long)(part % splits) * chunk, (long long)p.vocab) : 0;
+    const int n = live ? std::min((long long)chunk, (long long)p.vocab - lo) : 0;
+    const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+    const f32x4 a = live ? q.row[2 * (size_t)r] : none, b = live ? q.row[2 * (size_t)r + 1] : none;
+    const bool zero = b[3] == 0.f;
+    T* out = grad + (live ? (size_t)r * p.vocab + lo : 0);
+    const T* x = reinterpret_cast<const T*>(p.x) + (live ? row_offset(p, r) + lo : 0);
+    if (zero) {
+      store_zeros<T, TPR>(out, n, t);
+    } else {
+      const f32x4 k = {a[0], a[1] * scale, 0.f, 0.f};
+      const int head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+      const int nv = (n - head) / VEC, behind = head + nv * VEC;
+      const u32x4* v = reinterpret_cast<const u32x4*>(x + head);
+      u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
+      for (int i = t; i < nv; i += TPR) o[i] = gradient_vector<T, false>(v[i], k, p.c);
+      if (t < head) out[t] = (T)gradient_entry<false>((float)x[t], k, p.c);
+      if (t < n - behind) out[behind + t] = (T)gradient_entry<false>((float)x[behind + t], k, p.c);
+    }
+    __syncthreads();                                            // a listed element is written twice, in this order
+    if (!zero) patch_list<T>(p, q, r, a, b, scale, lo, n, x, out, t, TPR);
   }
-  __syncthreads();                                              // a listed element is written twice, in this order
-  if (!zero) patch_list<T>(p, q, r, a, b, scale, lo, n, x, out, t, TPR);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------
@@ -338,8 +326,8 @@ int launch_list_grad_t(const char* who, const Logits& p, const ListIn& q, const 
   const int tpr = bytes <= 4096 ? 64 : NT;
   const int chunk = bytes <= 4096 ? p.vocab : 16384 / (int)sizeof(T);
   const int splits = (int)st::cdivll(p.vocab, chunk);
-  const long long blocks = st::cdivll((long long)p.rows * splits, NT / tpr);
-  if (blocks > 0x7fffffffLL) return st::fail(ST_ERR_BAD_ARG, "%s: too many rows", who);
+  // a launch that may have nothing to do is kept small
+  const long long blocks = std::min<long long>(st::cdivll((long long)p.rows * splits, NT / tpr), skip ? 4096 : 0x7fffffffLL);
   if (tpr == 64) hipLaunchKernelGGL((list_grad_kernel<T, 64>), dim3((unsigned)blocks), dim3(NT), 0, s, p, q, gout, skip, splits, chunk, (T*)grad);
   else hipLaunchKernelGGL((list_grad_kernel<T, NT>), dim3((unsigned)blocks), dim3(NT), 0, s, p, q, gout, skip, splits, chunk, (T*)grad);
   return st::check_launch(who);
@@ -349,7 +337,7 @@ int launch_list_grad_t(const char* who, const Logits& p, const ListIn& q, const 
 
 extern "C" size_t st_distill_workspace_bytes(long long rows) {
   if (rows <= 0 || rows > 0x7fffffffLL) return 0;
-  return sums_bytes(rows) + align256((size_t)rows * sizeof(ListSum));
+  return sums_bytes(rows);
 }
 
 extern "C" int st_distill_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer, long long s_inner, int vocab,
@@ -373,13 +361,11 @@ extern "C" int st_distill_loss_fwd(const void* x, int dtype, long long rows, lon
   q.mask = mask;
   q.tail = tail;
   q.scale = scale;
-  q.sum = w.take<ListSum>((size_t)rows);
   q.row = reinterpret_cast<f32x4*>(row_grad);
-  const unsigned blocks = (unsigned)std::min<long long>(2048, st::cdivll(rows, NT / 64));
-  u.blocks = (int)std::min<long long>(std::min<unsigned>(COUNT_BLOCKS, blocks), st::cdivll(rows, 1024));
+  u.blocks = (int)std::min<long long>(COUNT_BLOCKS, st::cdivll(rows, 4096));
+  if (mask) hipLaunchKernelGGL(count_mask_kernel, dim3(u.blocks), dim3(1024), 0, s, mask, u);
   return with_type(dtype, [&](auto type) {
     using T = decltype(type);
-    hipLaunchKernelGGL(list_sums_kernel<T>, dim3(blocks), dim3(NT), 0, s, p, q, u);
     const int words = (vocab + Type<T>::VEC + 31) / 32;
     const int launched = with_shape((long long)vocab * (long long)sizeof(T), [&](auto shape) -> int {
       using S = decltype(shape);

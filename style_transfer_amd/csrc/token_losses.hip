@@ -23,9 +23,9 @@ __device__ __forceinline__ float load_one(const void* base, long long i) {
 template <typename T>
 __device__ __forceinline__ void write_row(const Logits& p, unsigned r, long long label, const Part& q, float* logp, float* entropy,
                                           f32x4* state) {
-  const RowStat st = finish(q, p.c, p.tau);
+  const RowStat st = finish(q, p);
   float lp = NAN, h = st.h, inv = st.inv_ts;
-  if (label >= 0 && label < p.vocab) lp = (float)log_prob(load_one<T>(p.x, row_offset(p, r) + label), st, p.tau);
+  if (label >= 0 && label < p.vocab) lp = (float)log_prob(load_one<T>(p.x, row_offset(p, r) + label), st, p);
   else inv = NAN;                                              // a label outside the vocabulary: visible, never an access
   logp[r] = lp;
   if (entropy) entropy[r] = h;
@@ -85,7 +85,6 @@ struct StatsOut {
 
 template <typename T, int TPR>
 __global__ __launch_bounds__(NT) void stats_kernel(Logits p, int splits, int chunk, StatsOut o) {
-  constexpr int WPR = TPR / 64;                                // waves of a part
   __shared__ Part red[NT / 64];
   const int t = threadIdx.x % TPR;
   const unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
@@ -97,14 +96,7 @@ __global__ __launch_bounds__(NT) void stats_kernel(Logits p, int splits, int chu
   if (live && label != p.ignore) {
     const int lo = std::min((long long)sp * chunk, (long long)p.vocab), hi = std::min((long long)lo + chunk, (long long)p.vocab);
     const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r) + lo;
-    Part q = wave_join(stream_part<T, TPR>(x, hi - lo, p.c, t), p.c);
-    if (WPR > 1) {                                             // the whole block has this row: the barriers are uniform
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = q;
-      __syncthreads();
-      q = red[0];
-#pragma unroll
-      for (int w = 1; w < WPR; ++w) q = join(q, red[w], p.c);
-    }
+    const Part q = row_join<TPR>(stream_part<T, TPR>(x, hi - lo, p.c, t), p.c, red);     // TPR > 64: one row, so the barrier is uniform
     if (t == 0) {
       if (splits > 1) o.parts[part] = f32x4{q.m, q.s, q.w, 0.f};
       else write_row<T>(p, r, label, q, o.logp, o.entropy, o.state);
@@ -169,9 +161,10 @@ __device__ __forceinline__ void stream_gradient(const T* x, T* out, int n, const
   const int nv = (n - head) / VEC, behind = head + nv * VEC;
   const u32x4* v = reinterpret_cast<const u32x4*>(x + head);
   u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
-  for (int i = t; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH>(v[i], k, c, at - head - i * VEC);
-  if (t < head) out[t] = gradient_one<T, BOTH>((float)x[t], k, c, t == at);
-  if (t < n - behind) out[behind + t] = gradient_one<T, BOTH>((float)x[behind + t], k, c, behind + t == at);
+  for (int i = t; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH>(v[i], k, c);
+  const int j = t < head ? t : behind + t - head;               // the thread's element before or behind the vectors
+  if (j < n && (t < head || j >= behind)) out[j] = (T)gradient_entry<BOTH>((float)x[j], k, c);
+  store_label<T, TPR>(x, out, n, head, nv, k, c, at, t);
 }
 
 template <typename T, int TPR>
@@ -179,22 +172,24 @@ __global__ __launch_bounds__(NT) void grad_kernel(Logits p, GradIn g, int splits
   const float scale = g.gout ? g.gout[0] : 1.f;
   if (g.skip_if_one && scale == 1.f) return;
   const int t = threadIdx.x % TPR;
-  const unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
-  const unsigned r = (unsigned)(part / splits);
-  if (r >= p.rows) return;
-  const int lo = std::min((long long)(part % splits) * chunk, (long long)p.vocab);
-  const int n = std::min((long long)chunk, (long long)p.vocab - lo);
-  const long long label = load_index(p.labels, p.labels64, r);
-  const RowGrad k = row_grad(p, g, r, scale, label != p.ignore);
-  T* out = grad + (size_t)r * p.vocab + lo;
-  const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r) + lo;
-  if (k[1] == 0.f && k[2] == 0.f && k[3] == 0.f) {
-    store_zeros<T, TPR>(out, n, t);
-    return;
+  const unsigned long long parts = (unsigned long long)p.rows * splits;
+  for (unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR; part < parts;
+       part += (unsigned long long)gridDim.x * (NT / TPR)) {
+    const unsigned r = (unsigned)(part / splits);
+    const int lo = std::min((long long)(part % splits) * chunk, (long long)p.vocab);
+    const int n = std::min((long long)chunk, (long long)p.vocab - lo);
+    const long long label = load_index(p.labels, p.labels64, r);
+    const RowGrad k = row_grad(p, g, r, scale, label != p.ignore);
+    T* out = grad + (size_t)r * p.vocab + lo;
+    const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r) + lo;
+    if (k[1] == 0.f && k[2] == 0.f && k[3] == 0.f) {
+      store_zeros<T, TPR>(out, n, t);
+      continue;
+    }
+    const int at = (int)std::max(-1ll, std::min(label - lo, (long long)n));
+    if (k[2] == 0.f) stream_gradient<T, TPR, false>(x, out, n, k, p.c, at, t);
+    else stream_gradient<T, TPR, true>(x, out, n, k, p.c, at, t);
   }
-  const int at = (int)std::max(-1ll, std::min(label - lo, (long long)n));
-  if (k[2] == 0.f) stream_gradient<T, TPR, false>(x, out, n, k, p.c, at, t);
-  else stream_gradient<T, TPR, true>(x, out, n, k, p.c, at, t);
 }
 
 // ---- preference loss ---------------------------------------------------------------------------------------------------
@@ -212,61 +207,66 @@ struct PrefIn {
   RowGrad* row;              // null without a gradient
 };
 
-__device__ __forceinline__ double log1p_exp(double v) { return v > 0 ? v + log1p(exp(-v)) : log1p(exp(v)); }
-
-// A block a pair: the two sums in fp64, the pair's loss and its slope, the rows' coefficients; the last block takes the mean.
+// A block a pair: the two sums in fp64, the pair's loss and its slope (first wave), the rows' coefficients.
 __global__ __launch_bounds__(1024) void pref_kernel(Logits p, PrefIn q) {
   __shared__ double red[16];
+  __shared__ double slopes[2];
   const unsigned pairs = q.seq.count / 2, pair = blockIdx.x;
-  double ratio[2];
-  double inv[2];
+  double sum[2], n[2];
+  unsigned start[2], end[2];
   for (int side = 0; side < 2; ++side) {
-    unsigned start, end;
-    sequence(q.seq, pair + side * pairs, start, end);
-    double sum = 0, n = 0;
-    for (unsigned r = start + threadIdx.x; r < end; r += blockDim.x) {
-      sum += (double)q.logp[r];
-      if (load_index(p.labels, p.labels64, r) != p.ignore) n += 1;
+    sequence(q.seq, pair + side * pairs, start[side], end[side]);
+    sum[side] = n[side] = 0;
+    for (unsigned r = start[side] + threadIdx.x; r < end[side]; r += 1024) {
+      sum[side] += (double)q.logp[r];
+      n[side] += load_index(p.labels, p.labels64, r) != p.ignore;
     }
-    sum = block_sum64(sum, red);
-    n = q.average ? block_sum64(n, red) : 1.0;
-    inv[side] = n > 0 ? 1.0 / n : 0.0;
-    ratio[side] = sum * (n > 0 ? 1.0 / n : 1.0) - (q.ref ? (double)q.ref[pair + side * pairs] : 0.0);
+    sum[side] = block_sum64(sum[side], red);
+    n[side] = q.average ? block_sum64(n[side], red) : 1.0;
   }
-  const double h = ratio[0] - ratio[1], z = q.beta * h;
-  double loss, slope;
-  if (q.kind == ST_PREF_SIGMOID) {
-    loss = (1 - q.smoothing) * log1p_exp(-z) + q.smoothing * log1p_exp(z);
-    slope = q.beta * (q.smoothing / (1 + exp(-z)) - (1 - q.smoothing) / (1 + exp(z)));
-  } else if (q.kind == ST_PREF_IPO) {
-    const double v = h - 0.5 / q.beta;
-    loss = v * v;
-    slope = 2 * v;
-  } else {
-    loss = z < 1 ? 1 - z : (z >= 1 ? 0.0 : z);                  // a NaN stays one
-    slope = z < 1 ? -q.beta : (z >= 1 ? 0.0 : z);
+  if (threadIdx.x < 64) {
+    double ratio[2], inv[2];
+    for (int side = 0; side < 2; ++side) {
+      inv[side] = n[side] > 0 ? 1.0 / n[side] : 0.0;
+      ratio[side] = sum[side] * (n[side] > 0 ? inv[side] : 1.0) - (q.ref ? (double)q.ref[pair + side * pairs] : 0.0);
+    }
+    const double h = ratio[0] - ratio[1], z = q.beta * h;
+    double loss, slope;
+    if (q.kind == ST_PREF_SIGMOID) {
+      const double e = exp(-fabs(z)), soft = log1p(e), small = e / (1 + e), large = 1 / (1 + e);
+      loss = (1 - q.smoothing) * (soft + fmax(-z, 0.0)) + q.smoothing * (soft + fmax(z, 0.0));
+      slope = q.beta * (q.smoothing * (z > 0 ? large : small) - (1 - q.smoothing) * (z > 0 ? small : large));
+      if (z != z) loss = slope = z;
+    } else if (q.kind == ST_PREF_IPO) {
+      const double v = h - 0.5 / q.beta;
+      loss = v * v;
+      slope = 2 * v;
+    } else {
+      loss = z < 1 ? 1 - z : (z >= 1 ? 0.0 : z);                // a NaN stays one
+      slope = z < 1 ? -q.beta : (z >= 1 ? 0.0 : z);
+    }
+    if (threadIdx.x < 2) {
+      const int side = threadIdx.x;
+      q.rewards[pair + side * pairs] = (float)(q.beta * ratio[side]);
+      slopes[side] = (side ? -slope : slope) * inv[side] * q.scale / pairs;
+      if (side == 0) q.each[pair] = loss;
+    }
   }
-  if (threadIdx.x == 0) {
-    q.each[pair] = loss;
-    q.rewards[pair] = (float)(q.beta * ratio[0]);
-    q.rewards[pairs + pair] = (float)(q.beta * ratio[1]);
-  }
+  __syncthreads();
   if (q.row)
     for (int side = 0; side < 2; ++side) {
-      unsigned start, end;
-      sequence(q.seq, pair + side * pairs, start, end);
-      const float a = (float)((side ? -slope : slope) * inv[side] * q.scale / pairs);
-      for (unsigned r = start + threadIdx.x; r < end; r += blockDim.x) {
+      const float a = (float)slopes[side], patch = (float)(slopes[side] * p.inv_tau);
+      for (unsigned r = start[side] + threadIdx.x; r < end[side]; r += 1024) {
         const f32x4 s = q.state[r];
         const bool counts = load_index(p.labels, p.labels64, r) != p.ignore && s[1] != 0.f;
-        q.row[r] = counts ? f32x4{s[0], -a * s[1], 0.f, a / (float)p.tau} : f32x4{0.f, 0.f, 0.f, 0.f};
+        q.row[r] = counts ? f32x4{s[0], -a * s[1], 0.f, patch} : f32x4{0.f, 0.f, 0.f, 0.f};
       }
     }
   if (last_block(q.counter)) {
-    double sum = 0;
-    for (unsigned i = threadIdx.x; i < pairs; i += blockDim.x) sum += __hip_atomic_load(q.each + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sum = block_sum64(sum, red);
-    if (threadIdx.x == 0) q.loss[0] = (float)(q.scale * sum / pairs);
+    double all = 0;
+    for (unsigned i = threadIdx.x; i < pairs; i += 1024) all += __hip_atomic_load(q.each + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    all = block_sum64(all, red);
+    if (threadIdx.x == 0) q.loss[0] = (float)(q.scale * all / pairs);
   }
 }
 
@@ -288,17 +288,31 @@ struct TokenTerms {
   double a;                  // d (surrogate + kl_coef KL) / d logp
 };
 
-__device__ __forceinline__ TokenTerms token_terms(double ratio, double d, const PolicyIn& q, double adv) {
+// exp(d) - 1 - d, which is all that is left of it near 0: its series up to |d| = 1
+__device__ __forceinline__ double kl_estimate(double d) {
+  if (!(fabs(d) <= 1.0)) {
+    const double e = (double)exp_wide(d);
+    return e == INFINITY ? e : e - 1.0 - d;
+  }
+  const float v = (float)d;
+  float s = 1.f / 39916800.f;                                   // sum of d^n / n! from n = 2; the term left out is below 2^-27 of it
+  constexpr float f[] = {1.f / 3628800.f, 1.f / 362880.f, 1.f / 40320.f, 1.f / 5040.f, 1.f / 720.f, 1.f / 120.f, 1.f / 24.f, 1.f / 6.f, 0.5f};
+#pragma unroll
+  for (int n = 0; n < 9; ++n) s = fmaf(s, v, f[n]);
+  return (double)(s * v) * d;
+}
+
+__device__ __forceinline__ TokenTerms token_terms(double log_ratio, double d, const PolicyIn& q, double adv) {
   TokenTerms t;
+  const double ratio = (double)exp_wide(log_ratio);
   const bool over = adv > 0 && ratio > 1 + q.high, under = adv < 0 && ratio < 1 - q.low;
   t.clipped = over || under;
   t.part = -adv * (over ? 1 + q.high : under ? 1 - q.low : ratio);
   t.a = t.clipped != 0 ? 0.0 : -adv * ratio;
   t.kl = 0;
   if (q.ref) {
-    const double e = expm1(d);                                  // exp(d) - 1 - d without its cancellation near 0
-    t.kl = e - d;
-    t.a -= q.kl * e;
+    t.kl = kl_estimate(d);
+    if (q.kl != 0) t.a -= q.kl * (t.kl + d);
   }
   return t;
 }
@@ -343,7 +357,6 @@ __global__ __launch_bounds__(1024) void count_kernel(Logits p, PolicyIn q, Sums 
   n = block_sum64(n, red);
   if (threadIdx.x == 0) {
     u.counted[blockIdx.x] = n;
-    if (blockIdx.x == 0) *u.counter = 0;
   }
 }
 
@@ -374,6 +387,7 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
   const bool inside = label >= 0 && label < p.vocab;
   const float x_label = inside ? (float)x[label] : NAN, old = q.old_logp[r], ref = q.ref ? q.ref[r] : 0.f;
   const float adv = q.adv[q.adv_per_sequence ? s : r];
+  const double share = counted_share(u);
   const int own = q.per_sequence ? q.count[s] : 1;
   Part m = row.stats(p.c);
   for (int i = t + S::NCH * TPR; i < row.nv; i += TPR) {
@@ -384,13 +398,13 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
   m = row_join<TPR>(m, p.c, red);
   f32x4 g{0.f, 0.f, 0.f, 0.f};
   if (TPR == 64 || threadIdx.x < 64) {
-    const double w = one_over_counted(u) / own;
-    const RowStat st = finish(m, p.c, p.tau);
-    const double logp = inside ? log_prob(x_label, st, p.tau) : NAN;
-    const TokenTerms k = token_terms(exp(logp - (double)old), (double)ref - logp, q, (double)adv);
+    const double w = one_over(share) / own;
+    const RowStat st = finish(m, p);
+    const double logp = inside ? log_prob(x_label, st, p) : NAN;
+    const TokenTerms k = token_terms(logp - (double)old, (double)ref - logp, q, (double)adv);
     if (st.inv_ts != 0.f) {
       const double a = q.scale * w * k.a, b = -q.scale * w * q.ent, over = (double)st.inv_ts;
-      g = f32x4{st.ref, (float)(-(a + b * ((double)st.h - st.ln_s)) * over), (float)(-b * LN2 * over), (float)(a / p.tau)};
+      g = f32x4{st.ref, (float)(-(a + b * ((double)st.h - st.ln_s)) * over), (float)(-b * LN2 * over), (float)(a * p.inv_tau)};
     }
     if (t == 0) {
       u.terms[r] = f32x4{(float)(w * k.part), (float)(w * k.kl), (float)(w * (double)st.h), (float)(w * k.clipped)};
@@ -450,8 +464,8 @@ int launch_grad_t(const char* who, const Logits& p, const GradIn& g, void* grad,
   const int tpr = bytes <= 4096 ? 64 : NT;
   const int chunk = bytes <= 4096 ? p.vocab : 16384 / (int)sizeof(T);
   const int splits = (int)st::cdivll(p.vocab, chunk);
-  const long long blocks = st::cdivll((long long)p.rows * splits, NT / tpr);
-  if (blocks > 0x7fffffffLL) return st::fail(ST_ERR_BAD_ARG, "%s: too many rows", who);
+  // a launch that may have nothing to do is kept small: 131072 blocks that end at once take 28 us, 4096 take 3
+  const long long blocks = std::min<long long>(st::cdivll((long long)p.rows * splits, NT / tpr), g.skip_if_one ? 4096 : 0x7fffffffLL);
   if (tpr == 64) hipLaunchKernelGGL((grad_kernel<T, 64>), dim3((unsigned)blocks), dim3(NT), 0, s, p, g, splits, chunk, (T*)grad);
   else hipLaunchKernelGGL((grad_kernel<T, NT>), dim3((unsigned)blocks), dim3(NT), 0, s, p, g, splits, chunk, (T*)grad);
   return st::check_launch(who);

@@ -42,7 +42,8 @@ struct Logits {
   int vocab;
   unsigned rows;
   float c;
-  double tau;
+  float eps_ln2;                         // c = (1 + eps) log2(e) / tau: eps ln2
+  double tau, inv_tau;
 };
 
 // what a gradient pass needs of a row (float4): reference m, alpha, gamma, patch
@@ -120,17 +121,74 @@ __device__ __forceinline__ void rebase(float& s, float& w, float m_old, float m_
   s *= f;
 }
 
-__device__ __forceinline__ Part join(Part a, Part b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  rebase(a.s, a.w, a.m, m, c);
-  rebase(b.s, b.w, b.m, m, c);
-  return {m, a.s + b.s, a.w + b.w};
+// Reductions over a wave by lane moves of the vector unit; the result is in every lane.  LANES = 16: over the first row of
+// sixteen lanes alone.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float lane_move(float v, float none) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(none), __float_as_uint(v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lane_move(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+constexpr int SHR1 = 0x111, SHR2 = 0x112, SHR4 = 0x114, SHR8 = 0x118, BCAST15 = 0x142, BCAST31 = 0x143;
+
+__device__ __forceinline__ float from_lane(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
+
+template <int LANES = 64>
+__device__ __forceinline__ float lanes_max(float v) {
+  v = fmaxf(v, lane_move<SHR1, 0xf>(v, -INFINITY));
+  v = fmaxf(v, lane_move<SHR2, 0xf>(v, -INFINITY));
+  v = fmaxf(v, lane_move<SHR4, 0xf>(v, -INFINITY));
+  v = fmaxf(v, lane_move<SHR8, 0xf>(v, -INFINITY));
+  if (LANES == 16) return from_lane(v, 15);
+  v = fmaxf(v, lane_move<BCAST15, 0xa>(v, -INFINITY));
+  v = fmaxf(v, lane_move<BCAST31, 0xc>(v, -INFINITY));
+  return from_lane(v, 63);
+}
+template <int LANES = 64>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += lane_move<SHR1, 0xf>(v, 0.f);
+  v += lane_move<SHR2, 0xf>(v, 0.f);
+  v += lane_move<SHR4, 0xf>(v, 0.f);
+  v += lane_move<SHR8, 0xf>(v, 0.f);
+  if (LANES == 16) return from_lane(v, 15);
+  v += lane_move<BCAST15, 0xa>(v, 0.f);
+  v += lane_move<BCAST31, 0xc>(v, 0.f);
+  return from_lane(v, 63);
+}
+__device__ __forceinline__ double lanes_sum(double v) {
+  v += lane_move<SHR1, 0xf>(v);
+  v += lane_move<SHR2, 0xf>(v);
+  v += lane_move<SHR4, 0xf>(v);
+  v += lane_move<SHR8, 0xf>(v);
+  v += lane_move<BCAST15, 0xa>(v);
+  v += lane_move<BCAST31, 0xc>(v);
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), 63) << 32 |
+                                        (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, 63));
 }
 
+// the parts of a wave's lanes (of its first 16), seen from their maximum
+template <int LANES = 64>
 __device__ __forceinline__ Part wave_join(Part p, float c) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    p = join(p, Part{__shfl_xor(p.m, off, 64), __shfl_xor(p.s, off, 64), __shfl_xor(p.w, off, 64)}, c);
+  const float m = lanes_max<LANES>(p.m);
+  rebase(p.s, p.w, p.m, m, c);
+  return {m, lanes_sum<LANES>(p.s), lanes_sum<LANES>(p.w)};
+}
+
+// The parts of a row's waves; every lane of the row's first wave gets the result (TPR > 64: through LDS, one barrier).
+template <int TPR>
+__device__ __forceinline__ Part row_join(Part p, float c, Part* red) {
+  p = wave_join(p, c);
+  if (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = p;
+    __syncthreads();
+    if (threadIdx.x < 64) p = wave_join<16>(threadIdx.x < TPR / 64 ? red[threadIdx.x] : Part{-INFINITY, 0.f, 0.f}, c);
+  }
   return p;
 }
 
@@ -179,27 +237,44 @@ struct RowStat {
   float ref;         // m, or 0
 };
 
-__device__ __forceinline__ RowStat finish(const Part& q, float c, double tau) {
+// ln of a positive number with the logarithm's own error, not that of a result of up to 88 in fp32
+__device__ __forceinline__ double ln_wide(float v) {
+  const float f = __builtin_amdgcn_frexp_mantf(v);              // [1/2, 1)
+  const int up = f < 0.70710678f;                               // to [0.7, 1.42): a small logarithm has a small error
+  return (double)(__builtin_amdgcn_frexp_expf(v) - up) * LN2 + (double)(__builtin_amdgcn_logf(up ? 2 * f : f) * (float)LN2);
+}
+
+// exp(v), relative error of about 2^-23 whatever the size of v
+__device__ __forceinline__ float exp_wide(double v) {
+  if (v != v) return (float)v;
+  const double y = fmax(fmin(v * (1.0 / LN2), 1000.0), -1000.0), k = rint(y);      // 2^1000 and 2^-1000 are inf and 0 here
+  return ldexpf(__builtin_amdgcn_exp2f((float)(y - k)), (int)k);
+}
+
+__device__ __forceinline__ float reciprocal(float v) {
+  const float r = __builtin_amdgcn_rcpf(v);
+  return fmaf(fmaf(-v, r, 1.f), r, r);
+}
+
+__device__ __forceinline__ RowStat finish(const Part& q, const Logits& p) {
   RowStat r;
   r.ref = finite_ref(q.m);
+  const float inv = reciprocal(q.s);
+  r.ln_s = ln_wide(fmaf(-p.eps_ln2, q.w, q.s));
+  r.h = (float)(r.ln_s - LN2 * (double)q.w * (double)inv);
+  r.inv_ts = (float)(p.inv_tau * (double)inv);
   if (q.s == 0.f) {
     r.ln_s = -INFINITY;
     r.h = 0.f;
     r.inv_ts = 0.f;
-    return r;
   }
-  const double eps = (double)c * LN2 * tau - 1.0;          // c = (1 + eps) log2(e) / tau
-  r.ln_s = log((double)q.s - eps * LN2 * (double)q.w);
-  r.h = (float)(r.ln_s - LN2 * (double)q.w / (double)q.s);
-  r.inv_ts = (float)(1.0 / (tau * (double)q.s));
   return r;
 }
 
 // natural logarithm of q at a logit
-__device__ __forceinline__ double log_prob(float x, const RowStat& r, double tau) {
-  return r.inv_ts == 0.f ? -INFINITY : ((double)x - (double)r.ref) / tau - r.ln_s;
+__device__ __forceinline__ double log_prob(float x, const RowStat& r, const Logits& p) {
+  return r.inv_ts == 0.f ? -INFINITY : ((double)x - (double)r.ref) * p.inv_tau - r.ln_s;
 }
-
 
 // Rows [start, end) of sequence s: cu[s], cu[s + 1] of a packed batch (clamped to the rows that are there), or the s-th
 // `inner` rows of a padded one.
@@ -223,8 +298,7 @@ __device__ __forceinline__ void sequence(const Sequences& q, unsigned s, unsigne
 }
 
 __device__ __forceinline__ double block_sum64(double v, double* red) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  v = lanes_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -246,31 +320,33 @@ __device__ __forceinline__ bool last_block(unsigned* counter) {
 }
 
 
-// ---- gradient entries: (alpha + gamma d_j) e_j, at the label + patch.  BOTH: gamma is not 0.  One form for every kernel that
-// writes them, with its roundings spelled out: a gradient computed again is the same to the bit. --------------------------------
+// ---- gradient entries: (alpha + gamma d_j) e_j, at the label + patch --------------------------------------------------------
+// BOTH: gamma is not 0 (the form with gamma = 0 has the same value).  One form for every kernel that writes them: a gradient
+// computed again is the same to the bit.
 template <bool BOTH>
 __device__ __forceinline__ float gradient_entry(float f, const f32x4& k, float c) {
   const float d = (f - k[0]) * c, e = __builtin_amdgcn_exp2f(d);
   return (BOTH ? fmaf(fmaxf(d, D_MIN), k[2], k[1]) : k[1]) * e;
 }
 template <typename T, bool BOTH>
-__device__ __forceinline__ T gradient_one(float f, const f32x4& k, float c, bool label) {
-#pragma clang fp contract(off)
-  const float g = gradient_entry<BOTH>(f, k, c);
-  return (T)(label ? g + k[3] : g);
-}
-template <typename T, bool BOTH>
-__device__ __forceinline__ u32x4 gradient_vector(const u32x4& w, const f32x4& k, float c, int label) {
-#pragma clang fp contract(off)
+__device__ __forceinline__ u32x4 gradient_vector(const u32x4& w, const f32x4& k, float c) {
   constexpr int VEC = Type<T>::VEC;
   float f[VEC];
   Type<T>::unpack(w, f);
 #pragma unroll
   for (int j = 0; j < VEC; ++j) f[j] = gradient_entry<BOTH>(f[j], k, c);
-  if (label >= 0 && label < VEC)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = j == label ? f[j] + k[3] : f[j];
   return Type<T>::pack(f);
+}
+// The label's entry, written by the thread that wrote it as any other before: its two stores keep their order.  `at` counts
+// from x, of which TPR threads hold the vectors behind the first `head` elements in turn and the rest as its first elements.
+template <typename T, int TPR>
+__device__ __forceinline__ void store_label(const T* x, T* out, int n, int head, int nv, const f32x4& k, float c, int at, int t) {
+#pragma clang fp contract(off)
+  constexpr int VEC = Type<T>::VEC;
+  if (at < 0 || at >= n) return;
+  const int in = at - head, behind = nv * VEC;
+  const int owner = in < 0 ? at : in < behind ? in / VEC % TPR : head + in - behind;
+  if (t == owner) out[at] = (T)(gradient_entry<true>((float)x[at], k, c) + k[3]);
 }
 
 // ---- a row held by its threads -------------------------------------------------------------------------------------------
@@ -323,6 +399,7 @@ struct Row {
       for (int j = 0; j < VEC; ++j) m = fmaxf(m, f[j]);
     }
     forget();
+    m = lanes_max(m);                                           // one reference for the wave, in a scalar register
     const float ref = finite_ref(m);
     Part p{m, 0.f, 0.f};
     add_up<1>(&extra, ref, c, p.s, p.w);
@@ -342,20 +419,21 @@ struct Row {
   }
 
   template <bool BOTH>
-  __device__ __forceinline__ void store_as(T* out, const f32x4& k, float c, int at) const {
+  __device__ __forceinline__ void store_as(T* out, const f32x4& k, float c) const {
     u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
 #pragma unroll
     for (int q = 0; q < NCH; ++q) {
       const int i = t + q * TPR;
-      if (i < nv) o[i] = gradient_vector<T, BOTH>(v[q], k, c, at - head - i * VEC);
+      if (i < nv) o[i] = gradient_vector<T, BOTH>(v[q], k, c);
     }
-    for (int i = t + NCH * TPR; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH>(body()[i], k, c, at - head - i * VEC);
-    if (extra_at >= 0) out[extra_at] = gradient_one<T, BOTH>(extra, k, c, extra_at == at);
+    for (int i = t + NCH * TPR; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH>(body()[i], k, c);
+    if (extra_at >= 0) out[extra_at] = (T)gradient_entry<BOTH>(extra, k, c);
   }
   __device__ __forceinline__ void store(T* out, const f32x4& k, float c, int at) {
     forget();
-    if (k[2] == 0.f) store_as<false>(out, k, c, at);
-    else store_as<true>(out, k, c, at);
+    if (k[2] == 0.f) store_as<false>(out, k, c);
+    else store_as<true>(out, k, c);
+    store_label<T, TPR>(x, out, n, head, nv, k, c, at, t);
   }
 };
 
@@ -371,27 +449,6 @@ __device__ __forceinline__ void store_zeros(T* out, int n, int t) {
   if (t < n - behind) out[behind + t] = (T)0.f;
 }
 
-__device__ __forceinline__ float first_lane(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
-
-// The parts of a row's waves; the result is in the first wave (TPR > 64: through LDS, one barrier).
-template <int TPR>
-__device__ __forceinline__ Part row_join(Part p, float c, Part* red) {
-  p = wave_join(p, c);
-  if (TPR > 64) {
-    constexpr int WAVES = TPR / 64;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = p;
-    __syncthreads();
-    if (threadIdx.x < 64) {
-      p = threadIdx.x < WAVES ? red[threadIdx.x] : Part{-INFINITY, 0.f, 0.f};
-#pragma unroll
-      for (int off = WAVES / 2; off > 0; off >>= 1)
-        p = join(p, Part{__shfl_xor(p.m, off, 64), __shfl_xor(p.s, off, 64), __shfl_xor(p.w, off, 64)}, c);
-    }
-  }
-  // the lanes' sums differ in the last bit (each rounds its own part first): the first lane's is the row's
-  return Part{first_lane(p.m), first_lane(p.s), first_lane(p.w)};
-}
-
 // ---- counts and sums over rows --------------------------------------------------------------------------------------------------
 // Up to 64 blocks count what the mean divides by; every row's wave adds up their counts itself (whole numbers: any order).
 constexpr int COUNT_BLOCKS = 64;
@@ -401,27 +458,30 @@ struct Sums {
   int blocks;                // of them used
   f32x4* terms;              // [rows]: a row's weighted terms
   double* partial;           // [4][COUNT_BLOCKS]
-  unsigned* counter;
   unsigned rows;
   float* loss;               // scale * (terms[0] + kl terms[1] - ent terms[2])
   float* stats;              // the four sums, or null
   double scale, kl, ent;
 };
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
-}
-
-// 1 / what counts, in every lane of a wave; 0 where nothing does
-__device__ __forceinline__ double one_over_counted(const Sums& q) {
+// A lane's share of what counts (asked for early), and 1 / their sum in every lane of a wave; 0 where nothing counts.
+__device__ __forceinline__ double counted_share(const Sums& q) {
   const int lane = threadIdx.x & 63;
-  const double n = wave_sum64(lane < q.blocks ? q.counted[lane] : 0.0);
+  return lane < q.blocks ? q.counted[lane] : 0.0;
+}
+__device__ __forceinline__ double one_over(double share) {
+  const double n = lanes_sum(share);
   return n > 0 ? 1.0 / n : 0.0;
 }
 
-// Adds the rows' terms in a fixed order; the last block adds the blocks' sums.
+__device__ __forceinline__ void write_sums(const Sums& q, const double* sum) {
+  q.loss[0] = (float)(q.scale * (sum[0] + (q.kl != 0 ? q.kl * sum[1] : 0.0) - (q.ent != 0 ? q.ent * sum[2] : 0.0)));
+  if (q.stats)
+    for (int k = 0; k < 4; ++k) q.stats[k] = (float)sum[k];
+}
+
+// Adds the rows' terms in a fixed order: one block all of them, or COUNT_BLOCKS blocks a share each and a block more behind
+// them.  (A last block that waits for the others' fences costs 13 us here: the gradient's lines are still in the caches.)
 static __global__ __launch_bounds__(1024) void sum_terms_kernel(Sums q) {
   __shared__ double red[16];
   double sum[4] = {0, 0, 0, 0};
@@ -429,23 +489,17 @@ static __global__ __launch_bounds__(1024) void sum_terms_kernel(Sums q) {
     const f32x4 v = q.terms[r];
     for (int k = 0; k < 4; ++k) sum[k] += (double)v[k];
   }
-  for (int k = 0; k < 4; ++k) {
-    sum[k] = block_sum64(sum[k], red);
-    if (threadIdx.x == 0) q.partial[k * COUNT_BLOCKS + blockIdx.x] = sum[k];
-  }
-  if (gridDim.x > 1) {
-    if (!last_block(q.counter)) return;
-    for (int k = 0; k < 4; ++k) {
-      const double v = threadIdx.x < gridDim.x
-                           ? __hip_atomic_load(q.partial + k * COUNT_BLOCKS + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-      sum[k] = block_sum64(v, red);
-    }
-  }
-  if (threadIdx.x == 0) {
-    q.loss[0] = (float)(q.scale * (sum[0] + (q.kl != 0 ? q.kl * sum[1] : 0.0) - (q.ent != 0 ? q.ent * sum[2] : 0.0)));
-    if (q.stats)
-      for (int k = 0; k < 4; ++k) q.stats[k] = (float)sum[k];
-  }
+  for (int k = 0; k < 4; ++k) sum[k] = block_sum64(sum[k], red);
+  if (threadIdx.x != 0) return;
+  if (gridDim.x == 1) write_sums(q, sum);
+  else
+    for (int k = 0; k < 4; ++k) q.partial[k * COUNT_BLOCKS + blockIdx.x] = sum[k];
+}
+
+static __global__ __launch_bounds__(64) void sum_partial_kernel(Sums q) {
+  double sum[4];
+  for (int k = 0; k < 4; ++k) sum[k] = lanes_sum(q.partial[k * COUNT_BLOCKS + threadIdx.x]);
+  if (threadIdx.x == 0) write_sums(q, sum);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
@@ -476,7 +530,9 @@ inline Logits make_logits(const void* x, long long rows, long long inner, long l
   p.vocab = vocab;
   p.rows = (unsigned)rows;
   p.tau = tau;
+  p.inv_tau = 1.0 / tau;
   p.c = (float)(1.0 / (LN2 * tau));
+  p.eps_ln2 = (float)(((double)p.c * LN2 * tau - 1.0) * LN2);
   return p;
 }
 
@@ -499,7 +555,6 @@ inline Sums make_sums(Space& w, long long rows, float* loss, float* stats, doubl
   Sums q{};
   q.counted = w.take<double>(COUNT_BLOCKS);
   q.partial = w.take<double>(4 * COUNT_BLOCKS);
-  q.counter = w.take<unsigned>(1);
   q.terms = w.take<f32x4>((size_t)rows);
   q.rows = (unsigned)rows;
   q.loss = loss;
@@ -510,10 +565,12 @@ inline Sums make_sums(Space& w, long long rows, float* loss, float* stats, doubl
   return q;
 }
 
-inline size_t sums_bytes(long long rows) { return align256(COUNT_BLOCKS * 8) * 5 + 256 + align256((size_t)rows * sizeof(f32x4)); }
+inline size_t sums_bytes(long long rows) { return align256(COUNT_BLOCKS * 8) * 5 + align256((size_t)rows * sizeof(f32x4)); }
 
 inline void launch_sum_terms(const Sums& q, hipStream_t s) {
-  hipLaunchKernelGGL(sum_terms_kernel, dim3(std::min<unsigned>(COUNT_BLOCKS, (unsigned)st::cdivll(q.rows, 4096))), dim3(1024), 0, s, q);
+  const bool one = q.rows <= 16384;                             // 16 rows a thread
+  hipLaunchKernelGGL(sum_terms_kernel, dim3(one ? 1 : COUNT_BLOCKS), dim3(1024), 0, s, q);
+  if (!one) hipLaunchKernelGGL(sum_partial_kernel, dim3(1), dim3(64), 0, s, q);
 }
 
 // Which of the row kernels takes a row of `bytes`: the smallest (threads, vectors a thread) that holds it, so that as many
