@@ -68,20 +68,20 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
   if (o.vref == -INFINITY) o.vref = 0.f;                        // no entry, or none with mass
   o.used = (int)lanes_sum((float)used);
   o.bad = __any(bad);
-  const float ref = finite_ref(o.m);
+  const Ref ref = make_ref(o.m, p.c);
   const double it = q.tail ? 1.0 : p.inv_tau;
   float s = 0.f, w = 0.f;
   double z = 0.0, gap = 0.0;
   for (int k = lane; k < q.k; k += 64) {
     const int j = entry_index(q, first + k, p.vocab);
     if (j < 0) continue;
-    const float f = (float)x[j], d = (f - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
+    const float f = (float)x[j], d = distance(f, ref, p.c), e = __builtin_amdgcn_exp2f(d);
     const double lv = ((double)q.val[first + k] - (double)o.vref) * it;
     const float ev = exp_wide(lv);
     s += e;
     w = fmaf(fmaxf(d, D_MIN), e, w);
     z += (double)ev;
-    if (ev != 0.f) gap += (double)ev * (lv - ((double)f - (double)ref) * p.inv_tau);
+    if (ev != 0.f) gap += (double)ev * (lv - ((double)f - (double)ref.m) * p.inv_tau);
   }
   o.s = lanes_sum(s);
   o.w = lanes_sum(w);
@@ -99,26 +99,49 @@ __global__ __launch_bounds__(1024) void count_mask_kernel(const unsigned char* m
   if (threadIdx.x == 0) u.counted[blockIdx.x] = n;
 }
 
-// Bits of the listed elements of [lo, lo + n), shifted so that a 16-byte vector's elements start at a multiple of VEC;
-// returns whether this thread met an index that was set before.
-__device__ __forceinline__ bool mark(uint32_t* bits, const ListIn& q, unsigned r, int lo, int n, int shift, int t, int threads) {
-  bool twice = false;
-  for (int k = t; k < q.k; k += threads) {
-    const long long j = load_index(q.idx, q.idx64, (size_t)r * q.k + k) - lo;
-    if (j < 0 || j >= n) continue;
-    const unsigned at = (unsigned)j + shift, bit = 1u << (at & 31);
-    twice |= (atomicOr(bits + (at >> 5), bit) & bit) != 0;
-  }
-  return twice;
-}
+// A bit for each element of a row, a word of a thread's vectors behind the other: the words of a row's threads lie side by
+// side, so that a wave reads them without conflicts, and 32 / VEC vectors cost a thread one read.  The elements outside the
+// vectors have the last word.
+template <typename T, int TPR>
+struct Marks {
+  static constexpr int VEC = Type<T>::VEC, PER = 32 / VEC, THREADS = TPR;      // PER: vectors of a word
+  uint32_t* bits;
 
-__device__ __forceinline__ bool marked(const uint32_t* bits, unsigned at) { return bits[at >> 5] >> (at & 31) & 1; }
+  static __host__ __device__ int words(int vocab) {             // of a row, whatever its alignment
+    const int slots = (vocab / VEC + TPR - 1) / TPR;
+    return (slots + PER - 1) / PER * TPR + 1;
+  }
+  // whether it was set before
+  __device__ __forceinline__ bool set(const Span<T, TPR>& row, int j, int last) const {
+    const int in = j - row.head, i = in / VEC;
+    const bool body = in >= 0 && i < row.nv;
+    const int slot = i / TPR, at = body ? slot / PER * TPR + i % TPR : last;
+    const uint32_t bit = 1u << (body ? slot % PER * VEC + in % VEC : row.owner(j));
+    return (atomicOr(bits + at, bit) & bit) != 0;
+  }
+  // the bits of the PER vectors from slot `slot` on (a multiple of PER)
+  __device__ __forceinline__ uint32_t word(int slot, int t) const { return bits[slot / PER * TPR + t]; }
+};
+
+// -inf in place of the listed elements of a vector that is read from memory
+template <typename M>
+struct Unlisted {
+  M marks;
+  template <typename R> __device__ __forceinline__ void operator()(const R& row, int i, float* f) const {
+    const int slot = i / M::THREADS;
+    const uint32_t on = marks.word(slot / M::PER * M::PER, row.t) >> (slot % M::PER * M::VEC) & ((1u << M::VEC) - 1);
+    if (on)
+#pragma unroll
+      for (int j = 0; j < M::VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
+  }
+};
 
 // The entries of a row's list that lie in [lo, lo + n), over the stream that wrote them as if they were off it.
 template <typename T>
 __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, unsigned r, const f32x4& a, const f32x4& b, float scale, int lo,
                                            int n, const T* x, T* out, int t, int threads) {
   const float cv = q.tail ? (float)(1.0 / LN2) : p.c;
+  const Ref ref = make_ref(a[2], p.c);
   const size_t first = (size_t)r * q.k;
   for (int k = t; k < q.k; k += threads) {
     const long long j = load_index(q.idx, q.idx64, first + k) - lo;
@@ -130,7 +153,7 @@ __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, uns
     } else {
       pk = __builtin_amdgcn_exp2f((q.val[first + k] - b[0]) * cv);
     }
-    const float e = __builtin_amdgcn_exp2f(((float)x[j] - a[2]) * p.c);
+    const float e = __builtin_amdgcn_exp2f(distance((float)x[j], ref, p.c));
     out[j] = (T)(scale * (a[3] * e - b[1] * pk));
   }
 }
@@ -139,7 +162,7 @@ __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, uns
 template <typename T>
 __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn& q, unsigned r, const T* x, ListSum o) {
   const size_t first = (size_t)r * q.k;
-  const float ref = finite_ref(o.m);
+  const Ref ref = make_ref(o.m, p.c);
   float s = 0, w = 0, n = 0;
   for (int k = threadIdx.x & 63; k < q.k; k += 64) {
     const int j = entry_index(q, first + k, p.vocab);
@@ -148,7 +171,7 @@ __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn
     if (again) {
       n += 1;
     } else if (j >= 0) {
-      const float d = ((float)x[j] - ref) * p.c, e = __builtin_amdgcn_exp2f(d);
+      const float d = distance((float)x[j], ref, p.c), e = __builtin_amdgcn_exp2f(d);
       s += e;
       w = fmaf(fmaxf(d, D_MIN), e, w);
     }
@@ -162,28 +185,26 @@ __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn
 // A row's loss (not yet times its weight) and coefficients, from the statistics off the list and the list's own sums.
 __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, const Part& off, const ListSum& o, double weight, bool repeated,
                                               f32x4& a, f32x4& b) {
-  const float ref = finite_ref(fmaxf(off.m, o.m)), ref_off = finite_ref(off.m), ref_list = finite_ref(o.m);
-  float s_off = off.s, w_off = off.w, s_list = o.s, w_list = o.w;
+  const Ref ref = make_ref(fmaxf(off.m, o.m), p.c), ref_off = make_ref(off.m, p.c);
+  // W off the list is not kept (it costs a sixth of the pass over the row): taken as if those elements sat at their reference
+  float s_off = off.s, w_off = 0.f, s_list = o.s, w_list = o.w;
   rebase(s_off, w_off, off.m, ref, p.c);
   rebase(s_list, w_list, o.m, ref, p.c);
   const float s = s_list + s_off, w = w_list + w_off;
-  const double ln_s = ln_wide(fmaf(-p.eps_ln2, w, s));
+  const double ln_z = logit_of(ref, p) + ln_wide(fmaf(-p.eps_ln2, w, s));              // ln of the sum of exp(x / tau)
   const double mass = q.tail ? o.z : o.z == 0 ? 0.0 : o.z / o.z;                       // 1, or NaN
   double loss = 0;
   if (mass != 0) {
-    loss = (q.tail ? o.gap : o.gap / o.z - (double)ln_wide((float)o.z)) + mass * (ln_s - ((double)ref_list - (double)ref) * p.inv_tau);
+    loss = (q.tail ? o.gap : o.gap / o.z - ln_wide((float)o.z)) + mass * (ln_z - (double)make_ref(o.m, p.c).m * p.inv_tau);
     if (s == 0.f) loss = INFINITY;
   }
   const double rest = q.tail && o.used < p.vocab ? (mass < 1 ? 1 - mass : mass >= 1 ? 0.0 : mass) : 0.0;
   const float inv = reciprocal(s), inv_off = reciprocal(off.s);
-  if (rest != 0) {
-    const double ln_off = ln_wide(fmaf(-p.eps_ln2, off.w, off.s)) + ((double)ref_off - (double)ref) * p.inv_tau;
-    loss += off.s == 0.f ? INFINITY : rest * (ln_wide((float)rest) - (ln_off - ln_s));
-  }
+  if (rest != 0) loss += off.s == 0.f ? INFINITY : rest * (ln_wide((float)rest) - (logit_of(ref_off, p) + ln_wide(off.s) - ln_z));
   const double gr = q.scale * weight * p.tau, total = mass + rest;
   const float on = s == 0.f ? 0.f : (float)(gr * total * (double)inv);
-  const double back = (double)__builtin_amdgcn_exp2f((ref_off - ref) * p.c);
-  a = f32x4{ref_off, s == 0.f || off.s == 0.f ? 0.f : (float)(gr * (total * (double)inv * back - rest * (double)inv_off)), ref, on};
+  const double back = (double)__builtin_amdgcn_exp2f(step(off.m, ref, p.c));
+  a = f32x4{ref_off.m, s == 0.f || off.s == 0.f ? 0.f : (float)(gr * (total * (double)inv * back - rest * (double)inv_off)), ref.m, on};
   b = f32x4{o.vref, s == 0.f || mass == 0 ? 0.f : (float)(q.tail ? gr : gr / o.z), repeated ? 1.f : 0.f, s == 0.f || total == 0 ? 0.f : 1.f};
   if (o.bad) {
     loss = NAN;
@@ -196,11 +217,12 @@ __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, 
 template <typename T, typename S>
 __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, Sums u, int words, T* __restrict__ grad) {
   constexpr int TPR = S::TPR, VEC = Type<T>::VEC;
+  using M = Marks<T, TPR>;
   extern __shared__ uint32_t all_bits[];
   __shared__ Part red[TPR / 64];
   __shared__ f32x4 told[2];
   const int t = threadIdx.x % TPR;
-  uint32_t* bits = all_bits + (threadIdx.x / TPR) * words;
+  const M marks{all_bits + (threadIdx.x / TPR) * words};
   const unsigned r = blockIdx.x * S::ROWS + threadIdx.x / TPR;
   const bool counts = r < p.rows && (!q.mask || q.mask[r]);
   const T* x = reinterpret_cast<const T*>(p.x) + (counts ? row_offset(p, r) : 0);
@@ -209,10 +231,14 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   Row<T, TPR, S::NCH> row;
   row.load(x, counts ? p.vocab : 0, t);                         // on their way while the bitmap is made
   const double share = q.mask ? counted_share(u) : 0.0;
-  const int shift = (VEC - row.head % VEC) % VEC;
-  for (int i = t; i < words; i += TPR) bits[i] = 0;
+  for (int i = t; i < words; i += TPR) marks.bits[i] = 0;
   __syncthreads();
-  bool twice = counts && mark(bits, q, r, 0, p.vocab, shift, t, TPR);
+  bool twice = false;
+  if (counts)
+    for (int k = t; k < q.k; k += TPR) {
+      const int j = entry_index(q, (size_t)r * q.k + k, p.vocab);
+      if (j >= 0) twice |= marks.set(row, j, words - 1);
+    }
   if (TPR == 64) {
     __syncthreads();
     twice = __any(twice);
@@ -220,32 +246,24 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
     twice = __syncthreads_or(twice);
   }
 #pragma unroll
-  for (int i = 0; i < S::NCH; ++i) {
-    const int at = t + i * TPR;
-    if (at >= row.nv) continue;
-    const unsigned bit = row.head + at * VEC + shift;
-    const uint32_t on = bits[bit >> 5] >> (bit & 31) & ((1u << VEC) - 1);
-    if (on) {
-      float f[VEC];
-      Type<T>::unpack(row.v[i], f);
+  for (int i = 0; i < S::NCH; i += M::PER) {
+    if (i >= row.slots) continue;
+    const uint32_t word = marks.word(i, t);
+    if (word == 0) continue;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
-      row.v[i] = Type<T>::pack(f);
+    for (int k = 0; k < M::PER && i + k < S::NCH; ++k) {
+      const uint32_t on = word >> (k * VEC) & ((1u << VEC) - 1);
+      if (on) {
+        float f[VEC];
+        Type<T>::unpack(row.v[i + k], f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
+        row.v[i + k] = Type<T>::pack(f);
+      }
     }
   }
-  if (row.extra_at >= 0 && marked(bits, row.extra_at + shift)) row.extra = -INFINITY;
-  Part m = row.stats(p.c);
-  for (int i = t + S::NCH * TPR; i < row.nv; i += TPR) {
-    float f[VEC];
-    Type<T>::unpack(row.body()[i], f);
-    const unsigned bit = row.head + i * VEC + shift;
-    const uint32_t on = bits[bit >> 5] >> (bit & 31) & ((1u << VEC) - 1);
-    if (on)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
-    take<VEC>(m, f, p.c);
-  }
-  m = row_join<TPR>(m, p.c, red);
+  if (row.extra_at() >= 0 && marks.bits[words - 1] >> t & 1) row.extra = -INFINITY;
+  const Part m = row_join<TPR>(row.template stats<false>(p.c, Unlisted<M>{marks}), p.c, red);
   f32x4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
   if ((TPR == 64 || threadIdx.x < 64) && r < p.rows) {
     float loss = 0.f;
@@ -286,7 +304,6 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
 template <typename T, int TPR>
 __global__ __launch_bounds__(NT) void list_grad_kernel(Logits p, ListIn q, const float* gout, int skip_if_one, int splits, int chunk,
                                                        T* __restrict__ grad) {
-  constexpr int VEC = Type<T>::VEC;
   const float scale = gout ? gout[0] : 1.f;
   if (skip_if_one && scale == 1.f) return;
   const int t = threadIdx.x % TPR;
@@ -305,14 +322,7 @@ __global__ __launch_bounds__(NT) void list_grad_kernel(Logits p, ListIn q, const
     if (zero) {
       store_zeros<T, TPR>(out, n, t);
     } else {
-      const f32x4 k = {a[0], a[1] * scale, 0.f, 0.f};
-      const int head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-      const int nv = (n - head) / VEC, behind = head + nv * VEC;
-      const u32x4* v = reinterpret_cast<const u32x4*>(x + head);
-      u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
-      for (int i = t; i < nv; i += TPR) o[i] = gradient_vector<T, false>(v[i], k, p.c);
-      if (t < head) out[t] = (T)gradient_entry<false>((float)x[t], k, p.c);
-      if (t < n - behind) out[behind + t] = (T)gradient_entry<false>((float)x[behind + t], k, p.c);
+      Span<T, TPR>(x, n, t).stream_all(out, f32x4{a[0], a[1] * scale, 0.f, 0.f}, make_ref(a[0], p.c), p.c);
     }
     __syncthreads();                                            // a listed element is written twice, in this order
     if (!zero) patch_list<T>(p, q, r, a, b, scale, lo, n, x, out, t, TPR);
@@ -366,9 +376,9 @@ extern "C" int st_distill_loss_fwd(const void* x, int dtype, long long rows, lon
   if (mask) hipLaunchKernelGGL(count_mask_kernel, dim3(u.blocks), dim3(1024), 0, s, mask, u);
   return with_type(dtype, [&](auto type) {
     using T = decltype(type);
-    const int words = (vocab + Type<T>::VEC + 31) / 32;
     const int launched = with_shape((long long)vocab * (long long)sizeof(T), [&](auto shape) -> int {
       using S = decltype(shape);
+      const int words = Marks<T, S::TPR>::words(vocab);
       const size_t lds = (size_t)words * 4 * S::ROWS;
       if (lds > MAX_PLAIN_LDS) {                                // the attribute is set once a device: to the most that any call needs
         static st::DynLdsOptIn opt_in;

@@ -44,9 +44,9 @@ template <typename T, int TPR>
 __device__ __forceinline__ Part stream_part(const T* x, int n, float c, int t) {
   constexpr int VEC = Type<T>::VEC;
   Part p{-INFINITY, 0.f, 0.f};
-  const int head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-  const int nv = (n - head) / VEC;
-  const u32x4* v = reinterpret_cast<const u32x4*>(x + head);
+  const Span<T, TPR> span(x, n, t);
+  const u32x4* v = span.body();
+  const int nv = span.nv;
   int i = t;
   for (; i + 3 * TPR < nv; i += 4 * TPR) {                     // four loads in flight
     u32x4 b[4];
@@ -62,13 +62,9 @@ __device__ __forceinline__ Part stream_part(const T* x, int n, float c, int t) {
     Type<T>::unpack(v[i], f);
     take<VEC>(p, f, c);
   }
-  if (t < head) {
-    const float f = (float)x[t];
-    take<1>(p, &f, c);
-  }
-  const int done = head + nv * VEC;
-  if (t < n - done) {
-    const float f = (float)x[done + t];
+  const int j = span.extra_at();
+  if (j >= 0) {
+    const float f = (float)x[j];
     take<1>(p, &f, c);
   }
   return p;
@@ -79,7 +75,6 @@ struct StatsOut {
   float* entropy;
   f32x4* state;
   f32x4* parts;          // [rows][splits], used where splits > 1
-  unsigned* counter;     // cleared for the loss kernel behind this one
   RowGrad* clear;        // row gradients that a loss kernel fills in for the rows it owns
 };
 
@@ -90,7 +85,6 @@ __global__ __launch_bounds__(NT) void stats_kernel(Logits p, int splits, int chu
   const unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
   const unsigned r = (unsigned)(part / splits);
   const int sp = (int)(part % splits);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && o.counter) *o.counter = 0;
   const bool live = r < p.rows;
   const long long label = live && p.labels ? load_index(p.labels, p.labels64, r) : p.ignore;
   if (live && label != p.ignore) {
@@ -149,22 +143,9 @@ __device__ __forceinline__ RowGrad row_grad(const Logits& p, const GradIn& g, un
   if (s[1] == 0.f) return v;
   v[0] = s[0];
   v[1] = -(a + b * s[2]) * s[1];
-  v[2] = -b * (float)LN2 * s[1];
-  v[3] = a / (float)p.tau;
+  v[2] = -b * (float)p.inv_ct * s[1];
+  v[3] = a * (float)p.inv_tau;
   return v;
-}
-
-template <typename T, int TPR, bool BOTH>
-__device__ __forceinline__ void stream_gradient(const T* x, T* out, int n, const RowGrad& k, float c, int at, int t) {
-  constexpr int VEC = Type<T>::VEC;
-  const int head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-  const int nv = (n - head) / VEC, behind = head + nv * VEC;
-  const u32x4* v = reinterpret_cast<const u32x4*>(x + head);
-  u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
-  for (int i = t; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH>(v[i], k, c);
-  const int j = t < head ? t : behind + t - head;               // the thread's element before or behind the vectors
-  if (j < n && (t < head || j >= behind)) out[j] = (T)gradient_entry<BOTH>((float)x[j], k, c);
-  store_label<T, TPR>(x, out, n, head, nv, k, c, at, t);
 }
 
 template <typename T, int TPR>
@@ -186,9 +167,10 @@ __global__ __launch_bounds__(NT) void grad_kernel(Logits p, GradIn g, int splits
       store_zeros<T, TPR>(out, n, t);
       continue;
     }
-    const int at = (int)std::max(-1ll, std::min(label - lo, (long long)n));
-    if (k[2] == 0.f) stream_gradient<T, TPR, false>(x, out, n, k, p.c, at, t);
-    else stream_gradient<T, TPR, true>(x, out, n, k, p.c, at, t);
+    const Span<T, TPR> part_of(x, n, t);
+    const Ref ref = make_ref(k[0], p.c);
+    part_of.stream_all(out, k, ref, p.c);
+    part_of.label(out, k, ref, p.c, (int)std::max(-1ll, std::min(label - lo, (long long)n)));
   }
 }
 
@@ -201,7 +183,6 @@ struct PrefIn {
   int kind, average;
   double beta, smoothing, scale;
   double* each;              // [P] workspace
-  unsigned* counter;
   float* loss;
   float* rewards;            // beta (L - ref) of each sequence
   RowGrad* row;              // null without a gradient
@@ -262,12 +243,15 @@ __global__ __launch_bounds__(1024) void pref_kernel(Logits p, PrefIn q) {
         q.row[r] = counts ? f32x4{s[0], -a * s[1], 0.f, patch} : f32x4{0.f, 0.f, 0.f, 0.f};
       }
     }
-  if (last_block(q.counter)) {
-    double all = 0;
-    for (unsigned i = threadIdx.x; i < pairs; i += 1024) all += __hip_atomic_load(q.each + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    all = block_sum64(all, red);
-    if (threadIdx.x == 0) q.loss[0] = (float)(q.scale * all / pairs);
-  }
+}
+
+__global__ __launch_bounds__(256) void pref_mean_kernel(PrefIn q) {
+  __shared__ double red[4];
+  const unsigned pairs = q.seq.count / 2;
+  double sum = 0;
+  for (unsigned i = threadIdx.x; i < pairs; i += 256) sum += q.each[i];
+  sum = block_sum64(sum, red);
+  if (threadIdx.x == 0) q.loss[0] = (float)(q.scale * sum / pairs);
 }
 
 // ---- clipped policy loss --------------------------------------------------------------------------------------------------
@@ -389,13 +373,7 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
   const float adv = q.adv[q.adv_per_sequence ? s : r];
   const double share = counted_share(u);
   const int own = q.per_sequence ? q.count[s] : 1;
-  Part m = row.stats(p.c);
-  for (int i = t + S::NCH * TPR; i < row.nv; i += TPR) {
-    float f[Type<T>::VEC];
-    Type<T>::unpack(row.body()[i], f);
-    take<Type<T>::VEC>(m, f, p.c);
-  }
-  m = row_join<TPR>(m, p.c, red);
+  const Part m = row_join<TPR>(row.template stats<true>(p.c, Whole{}), p.c, red);
   f32x4 g{0.f, 0.f, 0.f, 0.f};
   if (TPR == 64 || threadIdx.x < 64) {
     const double w = one_over(share) / own;
@@ -404,7 +382,7 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
     const TokenTerms k = token_terms(logp - (double)old, (double)ref - logp, q, (double)adv);
     if (st.inv_ts != 0.f) {
       const double a = q.scale * w * k.a, b = -q.scale * w * q.ent, over = (double)st.inv_ts;
-      g = f32x4{st.ref, (float)(-(a + b * ((double)st.h - st.ln_s)) * over), (float)(-b * LN2 * over), (float)(a * p.inv_tau)};
+      g = f32x4{st.ref, (float)(-(a + b * ((double)st.h - st.ln_s)) * over), (float)(-b * p.inv_ct * over), (float)(a * p.inv_tau)};
     }
     if (t == 0) {
       u.terms[r] = f32x4{(float)(w * k.part), (float)(w * k.kl), (float)(w * (double)st.h), (float)(w * k.clipped)};
@@ -489,7 +467,7 @@ extern "C" size_t st_token_workspace_bytes(int dtype, long long rows, int vocab,
   if (rows < 0 || sequences < 0) return 0;
   const size_t r = (size_t)rows, q = (size_t)sequences;
   // parts, log-probabilities, statistics, pairs' losses; or rows' terms and sequences' counts
-  return std::max(parts_bytes(rows, vocab, size_of(dtype)) + align256(r * 4) + align256(r * 16) + align256(q * 8) + 256,
+  return std::max(parts_bytes(rows, vocab, size_of(dtype)) + align256(r * 4) + align256(r * 16) + align256(q * 8),
                   sums_bytes(rows) + align256(q * 4));
 }
 
@@ -546,8 +524,6 @@ extern "C" int st_preference_loss_fwd(const void* x, int dtype, long long rows, 
   o.logp = w.take<float>((size_t)rows);
   o.state = w.take<f32x4>((size_t)rows);
   q.each = w.take<double>((size_t)pairs);
-  q.counter = w.take<unsigned>(1);
-  o.counter = q.counter;
   o.clear = reinterpret_cast<RowGrad*>(row_grad);
   q.seq = Sequences{cu_seqlens, 2u * (unsigned)pairs, (unsigned)inner, (unsigned)rows};
   q.logp = o.logp;
@@ -563,6 +539,7 @@ extern "C" int st_preference_loss_fwd(const void* x, int dtype, long long rows, 
   q.row = o.clear;
   if ((rc = launch_stats(who, dtype, p, o, s)) != ST_OK) return rc;
   hipLaunchKernelGGL(pref_kernel, dim3((unsigned)pairs), dim3(1024), 0, s, p, q);
+  hipLaunchKernelGGL(pref_mean_kernel, dim3(1), dim3(256), 0, s, q);
   return st::check_launch(who);
 }
 

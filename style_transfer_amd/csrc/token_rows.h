@@ -1,20 +1,25 @@
 // Shared device code of the losses over rows of logits (token_losses.hip, token_distill.hip) for gfx950.
 //
-// One row of logits x[0..V) at temperature tau, in the base-2 domain of the hardware's exponential:
+// One row of logits x[0..V) at temperature tau, in the base-2 domain of the hardware's exponential, seen from a reference m:
 //
-//   c = log2(e) / tau     m = max x     d_j = (x_j - m) c     e_j = 2^d_j     S = sum e_j     W = sum e_j d_j
-//   log q_j = ln2 d_j - ln S            entropy H = ln S - ln2 W / S
+//   c = log2(e) / tau     d_j = x_j c - m c     e_j = 2^d_j     S = sum e_j     W = sum e_j d_j
+//   log q_j = ln2 d_j - ln S                    entropy H = ln S - ln2 W / S
 //
 // Every loss here reaches x through the label's log-probability and the entropy, or through a short list of entries, so
 // every gradient row is   g_j = (alpha + gamma d_j) e_j   plus a few patched entries.
 //
-// The difference x - m comes before the factor c: the lowest value of a type used as a mask cannot overflow against
-// itself, and a row that holds nothing else is the uniform distribution that the formula gives.  A row of -inf only has
-// S = 0: no distribution, log-probability -inf, entropy 0, gradient 0.
+// m is any value near the maximum, not the maximum itself: a wave takes the largest of its first vectors, and where the rest
+// of the row lies so far above it that S leaves 2^80 it starts again with the maximum.  That saves a pass over the row, and
+// lets the exponentials begin while the row is still arriving.  m c is rounded once and then the same for everybody: d_j is
+// one fused multiply-add, and no error but its own.
 //
-// Sums of a row are fp32 per thread and over a fixed tree; what a row is reduced to is finished in fp64 (one wave a row),
-// because a sequence's sum of hundreds of log-probabilities is compared with another model's: c's own rounding (relative
-// 2^-25) shifts every term the same way, and W, which is d S / d ln c up to a factor, takes that shift out again.
+// Where |m c| reaches 1e30 ("low" rows: nothing but the lowest value of the type, as a mask leaves them) the difference comes
+// first, d_j = (x_j - m) c, which cannot overflow against itself: such a row is the uniform distribution that the formula
+// gives.  A row of -inf only has S = 0: no distribution, log-probability -inf, entropy 0, gradient 0.
+//
+// Sums of a row are fp32 per thread and over a fixed tree; what a row is reduced to is finished around fp64 sums (one wave a
+// row), because a sequence's sum of hundreds of log-probabilities is compared with another model's: c's own rounding
+// (relative 2^-25) shifts every term the same way, and W, which is d S / d ln c up to a factor, takes that shift out again.
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -43,7 +48,7 @@ struct Logits {
   unsigned rows;
   float c;
   float eps_ln2;                         // c = (1 + eps) log2(e) / tau: eps ln2
-  double tau, inv_tau;
+  double tau, inv_tau, inv_ct;           // 1 / tau, 1 / (c tau)
 };
 
 // what a gradient pass needs of a row (float4): reference m, alpha, gamma, patch
@@ -111,11 +116,34 @@ struct Part {
   float m, s, w;
 };
 
-__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+constexpr float LOW = 1e30f, FAR = 0x1p80f;
 
-// A part seen from another reference: d' = d + t, t = (m_old - m_new) c <= 0.
-__device__ __forceinline__ void rebase(float& s, float& w, float m_old, float m_new, float c) {
-  const float t = (m_old - finite_ref(m_new)) * c;
+// A reference and its product with c, rounded once (the pragma keeps a difference of two of them from being fused).
+struct Ref {
+  float m, mc;
+  bool low;
+};
+__device__ __forceinline__ Ref make_ref(float m, float c) {
+#pragma clang fp contract(off)
+  const float f = m == -INFINITY ? 0.f : m;
+  const float mc = f * c;
+  return {f, mc, !(fabsf(mc) < LOW)};
+}
+template <bool IS_LOW>
+__device__ __forceinline__ float distance(float x, const Ref& r, float c) {
+  return IS_LOW ? (x - r.m) * c : fmaf(x, c, -r.mc);
+}
+__device__ __forceinline__ float distance(float x, const Ref& r, float c) { return r.low ? distance<true>(x, r, c) : distance<false>(x, r, c); }
+
+// from an old reference to a new one; -inf where the old part is empty
+__device__ __forceinline__ float step(float m_old, const Ref& to, float c) {
+#pragma clang fp contract(off)
+  return to.low ? (m_old - to.m) * c : m_old * c - to.mc;
+}
+
+// A part seen from another reference: d' = d + t.
+__device__ __forceinline__ void rebase(float& s, float& w, float m_old, const Ref& to, float c) {
+  const float t = step(m_old, to, c);
   const float f = __builtin_amdgcn_exp2f(t);
   w = f * fmaf(fmaxf(t, D_MIN), s, w);
   s *= f;
@@ -176,7 +204,7 @@ __device__ __forceinline__ double lanes_sum(double v) {
 template <int LANES = 64>
 __device__ __forceinline__ Part wave_join(Part p, float c) {
   const float m = lanes_max<LANES>(p.m);
-  rebase(p.s, p.w, p.m, m, c);
+  rebase(p.s, p.w, p.m, make_ref(m, c), c);
   return {m, lanes_sum<LANES>(p.s), lanes_sum<LANES>(p.w)};
 }
 
@@ -195,46 +223,52 @@ __device__ __forceinline__ Part row_join(Part p, float c, Part* red) {
 // e_j and e_j d_j of N elements, each group of four summed by itself first: where one element is most of S, what it is
 // added to loses the small ones' last digits all in one direction, and a row of 131072 has hundreds of them a thread
 // (measured on rows with one such element: ln S 1.3e-6 too small on average with one running sum).
-template <int N>
-__device__ __forceinline__ void add_up(const float* x, float ref, float c, float& s, float& w) {
+// WANT_W: W as well.
+template <int N, bool IS_LOW, bool WANT_W>
+__device__ __forceinline__ void add_up(const float* x, const Ref& ref, float c, float& s, float& w) {
   float ss = 0.f, ww = 0.f;
 #pragma unroll
   for (int g = 0; g < N; g += 4) {
     float e[4], a[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float d = g + i < N ? (x[g + i < N ? g + i : 0] - ref) * c : -INFINITY;
+      const float d = g + i < N ? distance<IS_LOW>(x[g + i < N ? g + i : 0], ref, c) : -INFINITY;
       e[i] = __builtin_amdgcn_exp2f(d);
       a[i] = fmaxf(d, D_MIN);
     }
     const float s4 = (e[0] + e[1]) + (e[2] + e[3]);
-    const float w4 = fmaf(a[1], e[1], a[0] * e[0]) + fmaf(a[3], e[3], a[2] * e[2]);
     ss = g == 0 ? s4 : ss + s4;
-    ww = g == 0 ? w4 : ww + w4;
+    if (WANT_W) {
+      const float w4 = fmaf(a[1], e[1], a[0] * e[0]) + fmaf(a[3], e[3], a[2] * e[2]);
+      ww = g == 0 ? w4 : ww + w4;
+    }
   }
   s += ss;
-  w += ww;
+  if (WANT_W) w += ww;
 }
 
-// N more elements into a thread's part
-template <int N>
+// N more elements into a thread's part, whose reference is the largest that it has seen
+template <int N, bool WANT_W = true>
 __device__ __forceinline__ void take(Part& p, const float* x, float c) {
   float m = p.m;
 #pragma unroll
   for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+  const Ref ref = make_ref(m, c);
   if (m > p.m) {
-    rebase(p.s, p.w, p.m, m, c);
+    rebase(p.s, p.w, p.m, ref, c);
     p.m = m;
   }
-  add_up<N>(x, finite_ref(p.m), c, p.s, p.w);
+  if (ref.low) add_up<N, true, WANT_W>(x, ref, c, p.s, p.w);
+  else add_up<N, false, WANT_W>(x, ref, c, p.s, p.w);
 }
 
 // ---- what the logits of a row say once its parts are joined ----------------------------------------------------------------
 struct RowStat {
+  double z;          // the reference as a logit over tau
   double ln_s;       // ln S, with the rounding of c taken out
   float h;           // entropy
   float inv_ts;      // 1 / (tau S); 0 for a row without a distribution
-  float ref;         // m, or 0
+  float ref;
 };
 
 // ln of a positive number with the logarithm's own error, not that of a result of up to 88 in fp32
@@ -256,12 +290,17 @@ __device__ __forceinline__ float reciprocal(float v) {
   return fmaf(fmaf(-v, r, 1.f), r, r);
 }
 
+// what a reference is in x / tau: m c is rounded, and stands for itself
+__device__ __forceinline__ double logit_of(const Ref& r, const Logits& p) { return r.low ? (double)r.m * p.inv_tau : (double)r.mc * p.inv_ct; }
+
 __device__ __forceinline__ RowStat finish(const Part& q, const Logits& p) {
   RowStat r;
-  r.ref = finite_ref(q.m);
+  const Ref ref = make_ref(q.m, p.c);
   const float inv = reciprocal(q.s);
+  r.ref = ref.m;
+  r.z = logit_of(ref, p);
   r.ln_s = ln_wide(fmaf(-p.eps_ln2, q.w, q.s));
-  r.h = (float)(r.ln_s - LN2 * (double)q.w * (double)inv);
+  r.h = (float)(r.ln_s - p.inv_ct * (double)q.w * (double)inv);
   r.inv_ts = (float)(p.inv_tau * (double)inv);
   if (q.s == 0.f) {
     r.ln_s = -INFINITY;
@@ -273,7 +312,7 @@ __device__ __forceinline__ RowStat finish(const Part& q, const Logits& p) {
 
 // natural logarithm of q at a logit
 __device__ __forceinline__ double log_prob(float x, const RowStat& r, const Logits& p) {
-  return r.inv_ts == 0.f ? -INFINITY : ((double)x - (double)r.ref) * p.inv_tau - r.ln_s;
+  return r.inv_ts == 0.f ? -INFINITY : (double)x * p.inv_tau - r.z - r.ln_s;
 }
 
 // Rows [start, end) of sequence s: cu[s], cu[s + 1] of a packed batch (clamped to the rows that are there), or the s-th
@@ -307,79 +346,104 @@ __device__ __forceinline__ double block_sum64(double v, double* red) {
   return t;
 }
 
-// True in exactly one block: the last one to come here.  What the other blocks wrote before is visible to it.
-__device__ __forceinline__ bool last_block(unsigned* counter) {
-  __shared__ unsigned seen;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) seen = atomicAdd(counter, 1u);
-  __syncthreads();
-  const bool last = seen == gridDim.x - 1;
-  if (last) __threadfence();
-  return last;
-}
-
-
 // ---- gradient entries: (alpha + gamma d_j) e_j, at the label + patch --------------------------------------------------------
 // BOTH: gamma is not 0 (the form with gamma = 0 has the same value).  One form for every kernel that writes them: a gradient
 // computed again is the same to the bit.
-template <bool BOTH>
-__device__ __forceinline__ float gradient_entry(float f, const f32x4& k, float c) {
-  const float d = (f - k[0]) * c, e = __builtin_amdgcn_exp2f(d);
+template <bool BOTH, bool IS_LOW>
+__device__ __forceinline__ float gradient_entry(float f, const f32x4& k, const Ref& ref, float c) {
+  const float d = distance<IS_LOW>(f, ref, c), e = __builtin_amdgcn_exp2f(d);
   return (BOTH ? fmaf(fmaxf(d, D_MIN), k[2], k[1]) : k[1]) * e;
 }
-template <typename T, bool BOTH>
-__device__ __forceinline__ u32x4 gradient_vector(const u32x4& w, const f32x4& k, float c) {
+template <typename T, bool BOTH, bool IS_LOW>
+__device__ __forceinline__ u32x4 gradient_vector(const u32x4& w, const f32x4& k, const Ref& ref, float c) {
   constexpr int VEC = Type<T>::VEC;
   float f[VEC];
   Type<T>::unpack(w, f);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) f[j] = gradient_entry<BOTH>(f[j], k, c);
+  for (int j = 0; j < VEC; ++j) f[j] = gradient_entry<BOTH, IS_LOW>(f[j], k, ref, c);
   return Type<T>::pack(f);
 }
-// The label's entry, written by the thread that wrote it as any other before: its two stores keep their order.  `at` counts
-// from x, of which TPR threads hold the vectors behind the first `head` elements in turn and the rest as its first elements.
+
+// What a row, or a part of one, is for the threads that share it: 16-byte vectors aligned on the input, in turn, and the up
+// to 2 (VEC - 1) elements before and behind them, one for each of the first threads.
 template <typename T, int TPR>
-__device__ __forceinline__ void store_label(const T* x, T* out, int n, int head, int nv, const f32x4& k, float c, int at, int t) {
+struct Span {
+  static constexpr int VEC = Type<T>::VEC;
+  const T* x;
+  int n, t, head, nv;
+  __device__ __forceinline__ Span() {}
+  __device__ __forceinline__ Span(const T* row, int elements, int thread) : x(row), n(elements), t(thread) {
+    head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+    nv = (n - head) / VEC;
+  }
+  __device__ __forceinline__ const u32x4* body() const { return reinterpret_cast<const u32x4*>(x + head); }
+  __device__ __forceinline__ int extra_at() const {             // this thread's element outside the vectors, or -1
+    const int j = t < head ? t : t + nv * VEC;
+    return j < n && t < head + n - (head + nv * VEC) ? j : -1;
+  }
+  __device__ __forceinline__ int owner(int at) const {          // the thread that has element `at`
+    const int in = at - head;
+    return in < 0 ? at : in < nv * VEC ? in / VEC % TPR : at - nv * VEC;
+  }
+
+  // gradient of the vectors from `first` on and of the element outside them
+  template <bool BOTH, bool IS_LOW>
+  __device__ __forceinline__ void stream(T* out, const f32x4& k, const Ref& ref, float c, int first) const {
+    u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
+    for (int i = t + first; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH, IS_LOW>(body()[i], k, ref, c);
+    const int j = extra_at();
+    if (j >= 0) out[j] = (T)gradient_entry<BOTH, IS_LOW>((float)x[j], k, ref, c);
+  }
+  __device__ __forceinline__ void stream_all(T* out, const f32x4& k, const Ref& ref, float c) const {
+    if (ref.low) stream<true, true>(out, k, ref, c, 0);
+    else if (k[2] != 0.f) stream<true, false>(out, k, ref, c, 0);
+    else stream<false, false>(out, k, ref, c, 0);
+  }
+  // the label's entry, by the thread that wrote it as any other before: its two stores keep their order
+  __device__ __forceinline__ void label(T* out, const f32x4& k, const Ref& ref, float c, int at) const {
 #pragma clang fp contract(off)
-  constexpr int VEC = Type<T>::VEC;
-  if (at < 0 || at >= n) return;
-  const int in = at - head, behind = nv * VEC;
-  const int owner = in < 0 ? at : in < behind ? in / VEC % TPR : head + in - behind;
-  if (t == owner) out[at] = (T)(gradient_entry<true>((float)x[at], k, c) + k[3]);
-}
+    if (at < 0 || at >= n || t != owner(at)) return;
+    const float f = (float)x[at];
+    out[at] = (T)((ref.low ? gradient_entry<true, true>(f, k, ref, c) : gradient_entry<true, false>(f, k, ref, c)) + k[3]);
+  }
+};
 
 // ---- a row held by its threads -------------------------------------------------------------------------------------------
-// TPR threads hold up to TPR * NCH 16-byte vectors of a row in registers, so that its statistics and its gradient need one
-// read of memory; vectors beyond that (rows of more than 256 KB) are read again.  Vectors are aligned on the input; the up
-// to 2 (VEC - 1) elements before and behind them are one more register of the first threads.
+// TPR threads hold up to TPR * NCH vectors of a row in registers, so that its statistics and its gradient need one read of
+// memory; vectors beyond that (rows of more than 256 KB) are read again.  A wave passes over the vectors that none of its
+// lanes has.
 template <typename T> __device__ __forceinline__ u32x4 no_elements();       // -inf: adds nothing, changes no maximum
 template <> __device__ __forceinline__ u32x4 no_elements<float>() { return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }
 template <> __device__ __forceinline__ u32x4 no_elements<__bf16>() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
 template <> __device__ __forceinline__ u32x4 no_elements<_Float16>() { return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u}; }
 
+struct Whole {                // nothing of a vector is left out
+  template <typename R> __device__ __forceinline__ void operator()(const R&, int, float*) const {}
+};
+
 template <typename T, int TPR, int NCH>
-struct Row {
-  static constexpr int VEC = Type<T>::VEC;
+struct Row : Span<T, TPR> {
+  using Base = Span<T, TPR>;
+  using Base::VEC;
+  using Base::body;
+  using Base::n;
+  using Base::nv;
+  using Base::t;
+  using Base::x;
   u32x4 v[NCH];
-  float extra;               // the element `extra_at` (-1: none)
-  int extra_at, t, n, head, nv;
-  const T* x;
+  float extra;                // the element outside the vectors, -inf without one
+  int slots;                  // vectors of v that any lane of the wave has
 
-  __device__ __forceinline__ const u32x4* body() const { return reinterpret_cast<const u32x4*>(x + head); }
-
-  __device__ __forceinline__ void load(const T* row, int vocab, int thread) {
-    x = row;
-    n = vocab;
-    t = thread;
-    head = std::min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-    nv = (n - head) / VEC;
+  __device__ __forceinline__ void load(const T* row, int elements, int thread) {
+    static_cast<Base&>(*this) = Base(row, elements, thread);
+    const int first = __builtin_amdgcn_readfirstlane(t);
+    slots = nv > first ? (nv - first + TPR - 1) / TPR : 0;
     const u32x4* b = body();
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) v[i] = t + i * TPR < nv ? __builtin_nontemporal_load(b + t + i * TPR) : no_elements<T>();
-    const int behind = head + nv * VEC;
-    extra_at = t < head ? t : (t < head + n - behind ? behind + t - head : -1);
-    extra = extra_at >= 0 ? (float)x[extra_at] : -INFINITY;
+    for (int i = 0; i < NCH; ++i)
+      if (i < slots) v[i] = t + i * TPR < nv ? __builtin_nontemporal_load(b + t + i * TPR) : no_elements<T>();
+    const int at = this->extra_at();
+    extra = at >= 0 ? (float)x[at] : -INFINITY;
   }
 
   // Between two passes over the registers: what a pass made of them (twice as many floats of a 16-bit type) is made again
@@ -389,51 +453,69 @@ struct Row {
     for (int i = 0; i < NCH; ++i) asm volatile("" : "+v"(v[i]));
   }
 
-  __device__ __forceinline__ Part stats(float c) {
-    float m = extra;
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
+  // The thread's part of the row's statistics.  `leave_out(row, i, f)` puts -inf in place of what does not belong, in the
+  // elements f of vector i: it is asked for vectors that are read from memory, those in registers have it done.
+  template <bool WANT_W, typename F>
+  __device__ __forceinline__ Part stats(float c, F leave_out) {
+    float g = extra;
+    if (slots > 0) {
       float f[VEC];
-      Type<T>::unpack(v[i], f);
+      Type<T>::unpack(v[0], f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) m = fmaxf(m, f[j]);
+      for (int j = 0; j < VEC; ++j) g = fmaxf(g, f[j]);
     }
-    forget();
-    m = lanes_max(m);                                           // one reference for the wave, in a scalar register
-    const float ref = finite_ref(m);
-    Part p{m, 0.f, 0.f};
-    add_up<1>(&extra, ref, c, p.s, p.w);
+    g = lanes_max(g);                                           // one reference for the wave, in a scalar register
+    const Ref ref = make_ref(g, c);
+    Part p{ref.m, 0.f, 0.f};
+    if (!ref.low) {
+      add_up<1, false, WANT_W>(&extra, ref, c, p.s, p.w);
 #pragma unroll
-    for (int i = 0; i < NCH; i += 4) {
-      float s = 0.f, w = 0.f;
+      for (int i = 0; i < NCH; i += 4) {
+        float s = 0.f, w = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float f[VEC];
-        Type<T>::unpack(v[i + k], f);
-        add_up<VEC>(f, ref, c, s, w);
+        for (int k = 0; k < 4; ++k)
+          if (i + k < slots) {
+            float f[VEC];
+            Type<T>::unpack(v[i + k], f);
+            add_up<VEC, false, WANT_W>(f, ref, c, s, w);
+          }
+        p.s += s;
+        p.w += w;
       }
-      p.s += s;
-      p.w += w;
+    }
+    int from = NCH * TPR;
+    if (ref.low || !__all(p.s < FAR)) {                         // another reference is needed: again, with the largest so far
+      p = Part{-INFINITY, 0.f, 0.f};
+      take<1, WANT_W>(p, &extra, c);
+      from = 0;
+    }
+    for (int i = t + from; i < nv; i += TPR) {
+      float f[VEC];
+      Type<T>::unpack(body()[i], f);
+      leave_out(*this, i, f);
+      take<VEC, WANT_W>(p, f, c);
     }
     return p;
   }
 
   template <bool BOTH>
-  __device__ __forceinline__ void store_as(T* out, const f32x4& k, float c) const {
-    u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
+  __device__ __forceinline__ void store_as(T* out, const f32x4& k, const Ref& ref, float c) const {
+    u32x4_u* o = reinterpret_cast<u32x4_u*>(out + this->head);
 #pragma unroll
-    for (int q = 0; q < NCH; ++q) {
-      const int i = t + q * TPR;
-      if (i < nv) o[i] = gradient_vector<T, BOTH>(v[q], k, c);
-    }
-    for (int i = t + NCH * TPR; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH>(body()[i], k, c);
-    if (extra_at >= 0) out[extra_at] = (T)gradient_entry<BOTH>(extra, k, c);
+    for (int i = 0; i < NCH; ++i)
+      if (i < slots) {
+        const u32x4 w = gradient_vector<T, BOTH, false>(v[i], k, ref, c);
+        if (t + i * TPR < nv) o[t + i * TPR] = w;
+      }
+    this->template stream<BOTH, false>(out, k, ref, c, NCH * TPR);
   }
   __device__ __forceinline__ void store(T* out, const f32x4& k, float c, int at) {
     forget();
-    if (k[2] == 0.f) store_as<false>(out, k, c);
-    else store_as<true>(out, k, c);
-    store_label<T, TPR>(x, out, n, head, nv, k, c, at, t);
+    const Ref ref = make_ref(k[0], c);
+    if (ref.low) this->template stream<true, true>(out, k, ref, c, 0);
+    else if (k[2] != 0.f) store_as<true>(out, k, ref, c);
+    else store_as<false>(out, k, ref, c);
+    this->label(out, k, ref, c, at);
   }
 };
 
@@ -532,6 +614,7 @@ inline Logits make_logits(const void* x, long long rows, long long inner, long l
   p.tau = tau;
   p.inv_tau = 1.0 / tau;
   p.c = (float)(1.0 / (LN2 * tau));
+  p.inv_ct = 1.0 / ((double)p.c * tau);
   p.eps_ln2 = (float)(((double)p.c * LN2 * tau - 1.0) * LN2);
   return p;
 }
@@ -573,19 +656,21 @@ inline void launch_sum_terms(const Sums& q, hipStream_t s) {
   if (!one) hipLaunchKernelGGL(sum_partial_kernel, dim3(1), dim3(64), 0, s, q);
 }
 
-// Which of the row kernels takes a row of `bytes`: the smallest (threads, vectors a thread) that holds it, so that as many
-// rows as possible share a compute unit; the largest holds 256 KB (64 registers of 1024 threads) and reads again what is
-// beyond.  `kernel` is called with the two as integral constants.
+// Which of the row kernels takes a row of `bytes`: the fewest threads that hold it with 16 vectors each, so that as many
+// rows as possible share a compute unit, each in another phase of its work (16 vectors and about 50 more registers leave
+// room for 16 waves, 256 KB of rows); rows of up to 16 KB are a wave's and meet no barrier.  The largest reads again what is
+// beyond 256 KB.  `kernel` is called with the two numbers as a type.
 template <int A, int B> struct Shape {
-  static constexpr int TPR = A, NCH = B, BLOCK = A < NT ? NT : A, ROWS = BLOCK / A;
+  static constexpr int TPR = A, NCH = B, BLOCK = A == 64 ? 256 : A, ROWS = BLOCK / A;
 };
 template <typename F>
 auto with_shape(long long bytes, F kernel) {
   if (bytes <= 4 << 10) return kernel(Shape<64, 4>{});
-  if (bytes <= 16 << 10) return kernel(Shape<256, 4>{});
-  if (bytes <= 32 << 10) return kernel(Shape<256, 8>{});
-  if (bytes <= 64 << 10) return kernel(Shape<512, 8>{});
-  if (bytes <= 128 << 10) return kernel(Shape<1024, 8>{});
+  if (bytes <= 8 << 10) return kernel(Shape<64, 8>{});
+  if (bytes <= 16 << 10) return kernel(Shape<64, 16>{});
+  if (bytes <= 32 << 10) return kernel(Shape<128, 16>{});
+  if (bytes <= 64 << 10) return kernel(Shape<256, 16>{});
+  if (bytes <= 128 << 10) return kernel(Shape<512, 16>{});
   return kernel(Shape<1024, 16>{});
 }
 template <typename F>
