@@ -8,9 +8,9 @@
 // no digit of it where the student is sure of a listed token.  Entries that name the same token add up.
 //
 // One kernel holds a row in registers, with -inf in place of the listed elements, so that its statistics are those off the
-// list, and writes the gradient in two steps: the stream as if nothing were listed, then the K entries over it.  What the
-// list says by itself (K values, K gathered logits) is its first wave's work before that wave asks for its share of the row:
-// the other waves' share is on its way meanwhile, and the list needs none of the registers that the row will.
+// list, and writes the gradient in two steps: the stream as if nothing were listed, then the K entries over it.  A thread of
+// the row has one entry of the list (more where K is larger than the threads); entries and their logits are asked for before
+// the row, since loads return in order, and stay in registers until they are written.
 #include "token_rows.h"
 
 namespace {
@@ -20,12 +20,12 @@ using namespace st_token;
 constexpr int MAX_VOCAB = 1 << 20;       // the bitmap of a row: 128 KB of LDS
 constexpr size_t MAX_PLAIN_LDS = 48 << 10;   // dynamic LDS that a kernel gets without asking (64 KB with what it declares)
 
-// what the list of a row says by itself
+// what the list of a row, or a wave's part of it, says by itself
 struct ListSum {
-  float m, s, w;             // the listed logits' maximum, S and W of the listed tokens seen from it (once each entry)
-  float vref;                // the values' maximum; tail: 0
   double z;                  // sum of exp((v - vref) / tau); tail: the mass itself
   double gap;                // sum of exp((v - vref) / tau) ((v - vref) / tau - (x - m) / tau)
+  float m, s, w;             // the listed logits' maximum, S and W of the listed tokens seen from it (once each entry)
+  float vref;                // the values' maximum, -inf without any; tail: 0
   int used, bad;             // entries; any outside the vocabulary
 };
 
@@ -46,47 +46,87 @@ __device__ __forceinline__ int entry_index(const ListIn& q, size_t at, int vocab
   return j < 0 ? -1 : j >= vocab ? -2 : (int)j;
 }
 
-// a whole wave calls it
+struct Entry {
+  int j;                     // entry_index
+  float v, x;                // its value and its logit
+};
+
 template <typename T>
-__device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, unsigned r, const T* x) {
-  const int lane = threadIdx.x & 63;
-  const size_t first = (size_t)r * q.k;
+__device__ __forceinline__ Entry load_entry(const Logits& p, const ListIn& q, unsigned r, int k, const T* x) {
+  Entry e{-1, 0.f, -INFINITY};
+  if (k < q.k) {
+    e.j = entry_index(q, (size_t)r * q.k + k, p.vocab);
+    e.v = q.val[(size_t)r * q.k + k];
+    if (e.j >= 0) e.x = (float)x[e.j];
+  }
+  return e;
+}
+
+// A wave's part of the list: entry k of each lane (in `mine`), k + threads, ...  The whole wave calls it.
+template <typename T>
+__device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, unsigned r, const T* x, const Entry& mine, int k, int threads) {
   ListSum o;
   float m = -INFINITY, vref = -INFINITY;
   int used = 0, bad = 0;
-  for (int k = lane; k < q.k; k += 64) {
-    const int j = entry_index(q, first + k, p.vocab);
-    const float v = q.val[first + k];
-    bad |= j == -2;
-    if (j < 0) continue;
-    m = fmaxf(m, (float)x[j]);
-    vref = fmaxf(vref, v == v ? v : INFINITY);
-    ++used;
+  Entry e = mine;
+  for (int i = k;;) {
+    bad |= e.j == -2;
+    if (e.j >= 0) {
+      m = fmaxf(m, e.x);
+      vref = fmaxf(vref, e.v == e.v ? e.v : INFINITY);
+      ++used;
+    }
+    if ((i += threads) >= q.k) break;
+    e = load_entry(p, q, r, i, x);
   }
   o.m = lanes_max(m);
   o.vref = q.tail ? 0.f : lanes_max(vref);
-  if (o.vref == -INFINITY) o.vref = 0.f;                        // no entry, or none with mass
   o.used = (int)lanes_sum((float)used);
   o.bad = __any(bad);
   const Ref ref = make_ref(o.m, p.c);
-  const double it = q.tail ? 1.0 : p.inv_tau;
+  const double it = q.tail ? 1.0 : p.inv_tau, from = o.vref == -INFINITY ? 0.0 : (double)o.vref;
   float s = 0.f, w = 0.f;
   double z = 0.0, gap = 0.0;
-  for (int k = lane; k < q.k; k += 64) {
-    const int j = entry_index(q, first + k, p.vocab);
-    if (j < 0) continue;
-    const float f = (float)x[j], d = distance(f, ref, p.c), e = __builtin_amdgcn_exp2f(d);
-    const double lv = ((double)q.val[first + k] - (double)o.vref) * it;
-    const float ev = exp_wide(lv);
-    s += e;
-    w = fmaf(fmaxf(d, D_MIN), e, w);
-    z += (double)ev;
-    if (ev != 0.f) gap += (double)ev * (lv - ((double)f - (double)ref.m) * p.inv_tau);
+  e = mine;
+  for (int i = k;;) {
+    if (e.j >= 0) {
+      const float d = distance(e.x, ref, p.c), ex = __builtin_amdgcn_exp2f(d);
+      const double lv = ((double)e.v - from) * it;
+      const float ev = exp_wide(lv);
+      s += ex;
+      w = fmaf(fmaxf(d, D_MIN), ex, w);
+      z += (double)ev;
+      if (ev != 0.f) gap += (double)ev * (lv - ((double)e.x - (double)ref.m) * p.inv_tau);
+    }
+    if ((i += threads) >= q.k) break;
+    e = load_entry(p, q, r, i, x);
   }
   o.s = lanes_sum(s);
   o.w = lanes_sum(w);
   o.z = lanes_sum(z);
   o.gap = lanes_sum(gap);
+  return o;
+}
+
+// the waves' parts as one; lane i of the calling wave has wave i's (a part without entries: m = vref = -inf, the rest 0)
+__device__ __forceinline__ ListSum join_lists(const Logits& p, const ListIn& q, const ListSum& part) {
+  ListSum o;
+  o.m = lanes_max<16>(part.m);
+  o.vref = q.tail ? 0.f : lanes_max<16>(part.vref);
+  const Ref ref = make_ref(o.m, p.c);
+  float s = part.s, w = part.w;
+  rebase(s, w, part.m, ref, p.c);
+  // (v - vref) / tau and (x - m) / tau of the part's entries change by a and b
+  const bool any = part.z != 0;
+  const double a = !any || q.tail ? 0.0 : ((double)part.vref - (double)o.vref) * p.inv_tau;
+  const double b = any && part.m > -INFINITY ? ((double)part.m - (double)ref.m) * p.inv_tau : 0.0;
+  const double f = any ? (double)exp_wide(a) : 0.0;
+  o.s = lanes_sum<16>(s);
+  o.w = lanes_sum<16>(w);
+  o.z = lanes_sum(any ? f * part.z : 0.0);
+  o.gap = lanes_sum(any ? f * (part.gap + part.z * (a - b)) : 0.0);
+  o.used = (int)lanes_sum<16>((float)part.used);
+  o.bad = __any(part.bad);
   return o;
 }
 
@@ -136,25 +176,29 @@ struct Unlisted {
   }
 };
 
-// The entries of a row's list that lie in [lo, lo + n), over the stream that wrote them as if they were off it.
+// The entries of a row's list that lie in [lo, lo + n), over the stream that wrote them as if they were off it: entry t of
+// each thread (in `mine`), t + threads, ...  x and out are the row's beginning.
 template <typename T>
 __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, unsigned r, const f32x4& a, const f32x4& b, float scale, int lo,
-                                           int n, const T* x, T* out, int t, int threads) {
+                                           int n, const T* x, T* out, const Entry& mine, int t, int threads) {
   const float cv = q.tail ? (float)(1.0 / LN2) : p.c;
   const Ref ref = make_ref(a[2], p.c);
   const size_t first = (size_t)r * q.k;
-  for (int k = t; k < q.k; k += threads) {
-    const long long j = load_index(q.idx, q.idx64, first + k) - lo;
-    if (j < 0 || j >= n) continue;
-    float pk = 0.f;
-    if (b[2] != 0.f) {                                          // an index twice in this row: its entries' sum, in order
-      for (int i = 0; i < q.k; ++i)
-        if (load_index(q.idx, q.idx64, first + i) - lo == j) pk += __builtin_amdgcn_exp2f((q.val[first + i] - b[0]) * cv);
-    } else {
-      pk = __builtin_amdgcn_exp2f((q.val[first + k] - b[0]) * cv);
+  Entry e = mine;
+  for (int k = t;;) {
+    if (e.j >= lo && e.j - lo < n) {
+      float pk = 0.f;
+      if (b[2] != 0.f) {                                        // an index twice in this row: its entries' sum, in order
+        for (int i = 0; i < q.k; ++i)
+          if (entry_index(q, first + i, p.vocab) == e.j) pk += __builtin_amdgcn_exp2f((q.val[first + i] - b[0]) * cv);
+      } else {
+        pk = __builtin_amdgcn_exp2f((e.v - b[0]) * cv);
+      }
+      const float ex = __builtin_amdgcn_exp2f(distance(e.x, ref, p.c));
+      out[e.j] = (T)(scale * (a[3] * ex - b[1] * pk));
     }
-    const float e = __builtin_amdgcn_exp2f(distance((float)x[j], ref, p.c));
-    out[j] = (T)(scale * (a[3] * e - b[1] * pk));
+    if ((k += threads) >= q.k) break;
+    e = load_entry(p, q, r, k, x);
   }
 }
 
@@ -205,7 +249,7 @@ __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, 
   const float on = s == 0.f ? 0.f : (float)(gr * total * (double)inv);
   const double back = (double)__builtin_amdgcn_exp2f(step(off.m, ref, p.c));
   a = f32x4{ref_off.m, s == 0.f || off.s == 0.f ? 0.f : (float)(gr * (total * (double)inv * back - rest * (double)inv_off)), ref.m, on};
-  b = f32x4{o.vref, s == 0.f || mass == 0 ? 0.f : (float)(q.tail ? gr : gr / o.z), repeated ? 1.f : 0.f, s == 0.f || total == 0 ? 0.f : 1.f};
+  b = f32x4{o.vref == -INFINITY ? 0.f : o.vref, s == 0.f || mass == 0 ? 0.f : (float)(q.tail ? gr : gr / o.z), repeated ? 1.f : 0.f, s == 0.f || total == 0 ? 0.f : 1.f};
   if (o.bad) {
     loss = NAN;
     a[1] = a[3] = NAN;
@@ -214,37 +258,54 @@ __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, 
   return loss;
 }
 
+__device__ __forceinline__ void no_list(const ListIn& q, const Sums& u, unsigned r, int t) {
+  if (t == 0) u.terms[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (t < 2 && q.row) q.row[2 * (size_t)r + t] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
 template <typename T, typename S>
 __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, Sums u, int words, T* __restrict__ grad) {
   constexpr int TPR = S::TPR, VEC = Type<T>::VEC;
   using M = Marks<T, TPR>;
   extern __shared__ uint32_t all_bits[];
   __shared__ Part red[TPR / 64];
+  __shared__ ListSum lists[TPR / 64];
   __shared__ f32x4 told[2];
   const int t = threadIdx.x % TPR;
   const M marks{all_bits + (threadIdx.x / TPR) * words};
   const unsigned r = blockIdx.x * S::ROWS + threadIdx.x / TPR;
   const bool counts = r < p.rows && (!q.mask || q.mask[r]);
+  if (S::ROWS == 1 && !counts) {                                // the whole block
+    no_list(q, u, r, t);
+    if (grad) store_zeros<T, TPR>(grad + (size_t)r * p.vocab, p.vocab, t);
+    return;
+  }
   const T* x = reinterpret_cast<const T*>(p.x) + (counts ? row_offset(p, r) : 0);
-  ListSum list{};
-  if (counts && (TPR == 64 || threadIdx.x < 64)) list = sum_list(p, q, r, x);
-  Row<T, TPR, S::NCH> row;
-  row.load(x, counts ? p.vocab : 0, t);                         // on their way while the bitmap is made
-  const double share = q.mask ? counted_share(u) : 0.0;
+  Entry mine{-1, 0.f, -INFINITY};
+  if (counts) mine = load_entry(p, q, r, t, x);
   for (int i = t; i < words; i += TPR) marks.bits[i] = 0;
+  Row<T, TPR, S::NCH> row;
+  row.place(x, counts ? p.vocab : 0, t);
   __syncthreads();
   bool twice = false;
-  if (counts)
-    for (int k = t; k < q.k; k += TPR) {
+  if (counts && __builtin_amdgcn_readfirstlane(t) < q.k) {
+    if (mine.j >= 0) twice = marks.set(row, mine.j, words - 1);
+    for (int k = t + TPR; k < q.k; k += TPR) {
       const int j = entry_index(q, (size_t)r * q.k + k, p.vocab);
       if (j >= 0) twice |= marks.set(row, j, words - 1);
     }
+  }
+  row.load();
+  const double share = q.mask ? counted_share(u) : 0.0;
   if (TPR == 64) {
     __syncthreads();
     twice = __any(twice);
   } else {
     twice = __syncthreads_or(twice);
   }
+  ListSum list{0.0, 0.0, -INFINITY, 0.f, 0.f, -INFINITY, 0, 0};
+  if (counts && __builtin_amdgcn_readfirstlane(t) < q.k) list = sum_list(p, q, r, x, mine, t, TPR);
+  if (TPR > 64 && (threadIdx.x & 63) == 0) lists[threadIdx.x >> 6] = list;     // read behind row_join's barrier
 #pragma unroll
   for (int i = 0; i < S::NCH; i += M::PER) {
     if (i >= row.slots) continue;
@@ -265,13 +326,13 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   if (row.extra_at() >= 0 && marks.bits[words - 1] >> t & 1) row.extra = -INFINITY;
   const Part m = row_join<TPR>(row.template stats<false>(p.c, Unlisted<M>{marks}), p.c, red);
   f32x4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
-  if ((TPR == 64 || threadIdx.x < 64) && r < p.rows) {
-    float loss = 0.f;
-    if (counts) {
-      const double w = q.mask ? one_over(share) : 1.0 / u.rows;
-      if (twice) list = without_repeats(p, q, r, x, list);
-      loss = (float)(w * p.tau * p.tau * finish_list(p, q, m, list, w, twice, a, b));
-    }
+  if (!counts) {                                                // TPR = 64: a wave's row
+    if (r < p.rows) no_list(q, u, r, t);
+  } else if (TPR == 64 || threadIdx.x < 64) {
+    if (TPR > 64) list = join_lists(p, q, threadIdx.x < TPR / 64 ? lists[threadIdx.x] : ListSum{0.0, 0.0, -INFINITY, 0.f, 0.f, -INFINITY, 0, 0});
+    if (twice) list = without_repeats(p, q, r, x, list);
+    const double w = q.mask ? one_over(share) : 1.0 / u.rows;
+    const float loss = (float)(w * p.tau * p.tau * finish_list(p, q, m, list, w, twice, a, b));
     if (t == 0) {
       u.terms[r] = f32x4{loss, 0.f, 0.f, 0.f};
       if (q.row) {
@@ -297,7 +358,7 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
     else row.store(out, f32x4{a[0], a[1], 0.f, 0.f}, p.c, -1);
   }
   __syncthreads();                                              // a listed element is written twice, in this order
-  if (!zero) patch_list<T>(p, q, r, a, b, 1.f, 0, p.vocab, x, out, t, TPR);
+  if (!zero) patch_list<T>(p, q, r, a, b, 1.f, 0, p.vocab, x, out, mine, t, TPR);
 }
 
 // the gradient again, for another upstream gradient or a second time
@@ -325,7 +386,7 @@ __global__ __launch_bounds__(NT) void list_grad_kernel(Logits p, ListIn q, const
       Span<T, TPR>(x, n, t).stream_all(out, f32x4{a[0], a[1] * scale, 0.f, 0.f}, make_ref(a[0], p.c), p.c);
     }
     __syncthreads();                                            // a listed element is written twice, in this order
-    if (!zero) patch_list<T>(p, q, r, a, b, scale, lo, n, x, out, t, TPR);
+    if (!zero) patch_list<T>(p, q, r, a, b, scale, lo, n, x - lo, out - lo, load_entry(p, q, r, t, x - lo), t, TPR);
   }
 }
 

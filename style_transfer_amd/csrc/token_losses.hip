@@ -366,7 +366,8 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
   }
   const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r);
   Row<T, TPR, S::NCH> row;
-  row.load(x, p.vocab, t);
+  row.place(x, p.vocab, t);
+  row.load();
   // asked for before they are needed: they arrive with the row
   const bool inside = label >= 0 && label < p.vocab;
   const float x_label = inside ? (float)x[label] : NAN, old = q.old_logp[r], ref = q.ref ? q.ref[r] : 0.f;

@@ -434,8 +434,9 @@ struct Row : Span<T, TPR> {
   float extra;                // the element outside the vectors, -inf without one
   int slots;                  // vectors of v that any lane of the wave has
 
-  __device__ __forceinline__ void load(const T* row, int elements, int thread) {
-    static_cast<Base&>(*this) = Base(row, elements, thread);
+  __device__ __forceinline__ void place(const T* row, int elements, int thread) { static_cast<Base&>(*this) = Base(row, elements, thread); }
+
+  __device__ __forceinline__ void load() {
     const int first = __builtin_amdgcn_readfirstlane(t);
     slots = nv > first ? (nv - first + TPR - 1) / TPR : 0;
     const u32x4* b = body();
