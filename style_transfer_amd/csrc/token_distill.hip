@@ -24,7 +24,7 @@ constexpr size_t MAX_PLAIN_LDS = 48 << 10;   // dynamic LDS that a kernel gets w
 struct ListSum {
   double z;                  // sum of exp((v - vref) / tau); tail: the mass itself
   double gap;                // sum of exp((v - vref) / tau) ((v - vref) / tau - (x - m) / tau)
-  float m, s, w;             // the listed logits' maximum, S and W of the listed tokens seen from it (once each entry)
+  float m, s;                // the listed logits' maximum, S of the listed tokens seen from it (once each entry)
   float vref;                // the values' maximum, -inf without any; tail: 0
   int used, bad;             // entries; any outside the vocabulary
 };
@@ -81,11 +81,11 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
   }
   o.m = lanes_max(m);
   o.vref = q.tail ? 0.f : lanes_max(vref);
-  o.used = (int)lanes_sum((float)used);
+  o.used = q.k <= threads ? (int)__popcll(__ballot(used)) : (int)lanes_sum((float)used);
   o.bad = __any(bad);
   const Ref ref = make_ref(o.m, p.c);
   const double it = q.tail ? 1.0 : p.inv_tau, from = o.vref == -INFINITY ? 0.0 : (double)o.vref;
-  float s = 0.f, w = 0.f;
+  float s = 0.f;
   double z = 0.0, gap = 0.0;
   e = mine;
   for (int i = k;;) {
@@ -94,7 +94,6 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
       const double lv = ((double)e.v - from) * it;
       const float ev = exp_wide(lv);
       s += ex;
-      w = fmaf(fmaxf(d, D_MIN), ex, w);
       z += (double)ev;
       if (ev != 0.f) gap += (double)ev * (lv - ((double)e.x - (double)ref.m) * p.inv_tau);
     }
@@ -102,7 +101,6 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
     e = load_entry(p, q, r, i, x);
   }
   o.s = lanes_sum(s);
-  o.w = lanes_sum(w);
   o.z = lanes_sum(z);
   o.gap = lanes_sum(gap);
   return o;
@@ -114,15 +112,14 @@ __device__ __forceinline__ ListSum join_lists(const Logits& p, const ListIn& q, 
   o.m = lanes_max<16>(part.m);
   o.vref = q.tail ? 0.f : lanes_max<16>(part.vref);
   const Ref ref = make_ref(o.m, p.c);
-  float s = part.s, w = part.w;
-  rebase(s, w, part.m, ref, p.c);
+  float s = part.s, unused = 0.f;
+  rebase(s, unused, part.m, ref, p.c);
   // (v - vref) / tau and (x - m) / tau of the part's entries change by a and b
   const bool any = part.z != 0;
   const double a = !any || q.tail ? 0.0 : ((double)part.vref - (double)o.vref) * p.inv_tau;
   const double b = any && part.m > -INFINITY ? ((double)part.m - (double)ref.m) * p.inv_tau : 0.0;
   const double f = any ? (double)exp_wide(a) : 0.0;
   o.s = lanes_sum<16>(s);
-  o.w = lanes_sum<16>(w);
   o.z = lanes_sum(any ? f * part.z : 0.0);
   o.gap = lanes_sum(any ? f * (part.gap + part.z * (a - b)) : 0.0);
   o.used = (int)lanes_sum<16>((float)part.used);
@@ -163,17 +160,19 @@ struct Marks {
   __device__ __forceinline__ uint32_t word(int slot, int t) const { return bits[slot / PER * TPR + t]; }
 };
 
-// -inf in place of the listed elements of a vector that is read from memory
+// -inf in place of the listed elements.  (Their gradient is written as any other's first and then over it, so that the
+// registers keep the row as it is.)
 template <typename M>
 struct Unlisted {
   M marks;
-  template <typename R> __device__ __forceinline__ void operator()(const R& row, int i, float* f) const {
-    const int slot = i / M::THREADS;
-    const uint32_t on = marks.word(slot / M::PER * M::PER, row.t) >> (slot % M::PER * M::VEC) & ((1u << M::VEC) - 1);
+  int last;                  // the word of the elements outside the vectors
+  __device__ __forceinline__ void vector(int slot, int t, float* f) const {
+    const uint32_t on = marks.word(slot / M::PER * M::PER, t) >> (slot % M::PER * M::VEC) & ((1u << M::VEC) - 1);
     if (on)
 #pragma unroll
       for (int j = 0; j < M::VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
   }
+  __device__ __forceinline__ float extra(int t, float v) const { return t < 32 && marks.bits[last] >> t & 1 ? -INFINITY : v; }
 };
 
 // The entries of a row's list that lie in [lo, lo + n), over the stream that wrote them as if they were off it: entry t of
@@ -207,7 +206,7 @@ template <typename T>
 __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn& q, unsigned r, const T* x, ListSum o) {
   const size_t first = (size_t)r * q.k;
   const Ref ref = make_ref(o.m, p.c);
-  float s = 0, w = 0, n = 0;
+  float s = 0, n = 0;
   for (int k = threadIdx.x & 63; k < q.k; k += 64) {
     const int j = entry_index(q, first + k, p.vocab);
     bool again = false;
@@ -217,11 +216,9 @@ __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn
     } else if (j >= 0) {
       const float d = distance((float)x[j], ref, p.c), e = __builtin_amdgcn_exp2f(d);
       s += e;
-      w = fmaf(fmaxf(d, D_MIN), e, w);
     }
   }
   o.s = lanes_sum(s);
-  o.w = lanes_sum(w);
   o.used -= (int)lanes_sum(n);
   return o;
 }
@@ -230,12 +227,13 @@ __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn
 __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, const Part& off, const ListSum& o, double weight, bool repeated,
                                               f32x4& a, f32x4& b) {
   const Ref ref = make_ref(fmaxf(off.m, o.m), p.c), ref_off = make_ref(off.m, p.c);
-  // W off the list is not kept (it costs a sixth of the pass over the row): taken as if those elements sat at their reference
-  float s_off = off.s, w_off = 0.f, s_list = o.s, w_list = o.w;
-  rebase(s_off, w_off, off.m, ref, p.c);
-  rebase(s_list, w_list, o.m, ref, p.c);
-  const float s = s_list + s_off, w = w_list + w_off;
-  const double ln_z = logit_of(ref, p) + ln_wide(fmaf(-p.eps_ln2, w, s));              // ln of the sum of exp(x / tau)
+  // W is not kept here (it costs a sixth of the pass over the row): what it would take out of ln S, c's rounding times the mean
+  // distance from the reference, is below 1e-7, and these rows are not summed against another model's
+  float s_off = off.s, s_list = o.s, unused = 0.f;
+  rebase(s_off, unused, off.m, ref, p.c);
+  rebase(s_list, unused, o.m, ref, p.c);
+  const float s = s_list + s_off;
+  const double ln_z = logit_of(ref, p) + ln_wide(s);            // ln of the sum of exp(x / tau)
   const double mass = q.tail ? o.z : o.z == 0 ? 0.0 : o.z / o.z;                       // 1, or NaN
   double loss = 0;
   if (mass != 0) {
@@ -303,33 +301,15 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   } else {
     twice = __syncthreads_or(twice);
   }
-  ListSum list{0.0, 0.0, -INFINITY, 0.f, 0.f, -INFINITY, 0, 0};
+  ListSum list{0.0, 0.0, -INFINITY, 0.f, -INFINITY, 0, 0};
   if (counts && __builtin_amdgcn_readfirstlane(t) < q.k) list = sum_list(p, q, r, x, mine, t, TPR);
   if (TPR > 64 && (threadIdx.x & 63) == 0) lists[threadIdx.x >> 6] = list;     // read behind row_join's barrier
-#pragma unroll
-  for (int i = 0; i < S::NCH; i += M::PER) {
-    if (i >= row.slots) continue;
-    const uint32_t word = marks.word(i, t);
-    if (word == 0) continue;
-#pragma unroll
-    for (int k = 0; k < M::PER && i + k < S::NCH; ++k) {
-      const uint32_t on = word >> (k * VEC) & ((1u << VEC) - 1);
-      if (on) {
-        float f[VEC];
-        Type<T>::unpack(row.v[i + k], f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = on >> j & 1 ? -INFINITY : f[j];
-        row.v[i + k] = Type<T>::pack(f);
-      }
-    }
-  }
-  if (row.extra_at() >= 0 && marks.bits[words - 1] >> t & 1) row.extra = -INFINITY;
-  const Part m = row_join<TPR>(row.template stats<false>(p.c, Unlisted<M>{marks}), p.c, red);
+  const Part m = row_join<TPR>(row.template stats<false>(p.c, Unlisted<M>{marks, words - 1}), p.c, red);
   f32x4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
   if (!counts) {                                                // TPR = 64: a wave's row
     if (r < p.rows) no_list(q, u, r, t);
   } else if (TPR == 64 || threadIdx.x < 64) {
-    if (TPR > 64) list = join_lists(p, q, threadIdx.x < TPR / 64 ? lists[threadIdx.x] : ListSum{0.0, 0.0, -INFINITY, 0.f, 0.f, -INFINITY, 0, 0});
+    if (TPR > 64) list = join_lists(p, q, threadIdx.x < TPR / 64 ? lists[threadIdx.x] : ListSum{0.0, 0.0, -INFINITY, 0.f, -INFINITY, 0, 0});
     if (twice) list = without_repeats(p, q, r, x, list);
     const double w = q.mask ? one_over(share) : 1.0 / u.rows;
     const float loss = (float)(w * p.tau * p.tau * finish_list(p, q, m, list, w, twice, a, b));

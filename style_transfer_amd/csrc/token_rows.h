@@ -417,8 +417,9 @@ template <> __device__ __forceinline__ u32x4 no_elements<float>() { return u32x4
 template <> __device__ __forceinline__ u32x4 no_elements<__bf16>() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
 template <> __device__ __forceinline__ u32x4 no_elements<_Float16>() { return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u}; }
 
-struct Whole {                // nothing of a vector is left out
-  template <typename R> __device__ __forceinline__ void operator()(const R&, int, float*) const {}
+struct Whole {                // nothing of a row is left out
+  __device__ __forceinline__ void vector(int, int, float*) const {}
+  __device__ __forceinline__ float extra(int, float v) const { return v; }
 };
 
 template <typename T, int TPR, int NCH>
@@ -454,14 +455,16 @@ struct Row : Span<T, TPR> {
     for (int i = 0; i < NCH; ++i) asm volatile("" : "+v"(v[i]));
   }
 
-  // The thread's part of the row's statistics.  `leave_out(row, i, f)` puts -inf in place of what does not belong, in the
-  // elements f of vector i: it is asked for vectors that are read from memory, those in registers have it done.
+  // The thread's part of the row's statistics.  `leave_out` puts -inf in place of what does not belong: among the elements f of
+  // the thread's `slot`-th vector, and of the element outside the vectors.
   template <bool WANT_W, typename F>
-  __device__ __forceinline__ Part stats(float c, F leave_out) {
-    float g = extra;
+  __device__ __forceinline__ Part stats(float c, const F& leave_out) {
+    const float outside = leave_out.extra(t, extra);
+    float g = outside;
     if (slots > 0) {
       float f[VEC];
       Type<T>::unpack(v[0], f);
+      leave_out.vector(0, t, f);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) g = fmaxf(g, f[j]);
     }
@@ -469,7 +472,7 @@ struct Row : Span<T, TPR> {
     const Ref ref = make_ref(g, c);
     Part p{ref.m, 0.f, 0.f};
     if (!ref.low) {
-      add_up<1, false, WANT_W>(&extra, ref, c, p.s, p.w);
+      add_up<1, false, WANT_W>(&outside, ref, c, p.s, p.w);
 #pragma unroll
       for (int i = 0; i < NCH; i += 4) {
         float s = 0.f, w = 0.f;
@@ -478,22 +481,23 @@ struct Row : Span<T, TPR> {
           if (i + k < slots) {
             float f[VEC];
             Type<T>::unpack(v[i + k], f);
+            leave_out.vector(i + k, t, f);
             add_up<VEC, false, WANT_W>(f, ref, c, s, w);
           }
         p.s += s;
         p.w += w;
       }
     }
-    int from = NCH * TPR;
+    int from = NCH;
     if (ref.low || !__all(p.s < FAR)) {                         // another reference is needed: again, with the largest so far
       p = Part{-INFINITY, 0.f, 0.f};
-      take<1, WANT_W>(p, &extra, c);
+      take<1, WANT_W>(p, &outside, c);
       from = 0;
     }
-    for (int i = t + from; i < nv; i += TPR) {
+    for (int slot = from; t + slot * TPR < nv; ++slot) {
       float f[VEC];
-      Type<T>::unpack(body()[i], f);
-      leave_out(*this, i, f);
+      Type<T>::unpack(body()[t + slot * TPR], f);
+      leave_out.vector(slot, t, f);
       take<VEC, WANT_W>(p, f, c);
     }
     return p;
