@@ -46,33 +46,35 @@ __device__ __forceinline__ int entry_index(const ListIn& q, size_t at, int vocab
   return j < 0 ? -1 : j >= vocab ? -2 : (int)j;
 }
 
+template <typename T>
 struct Entry {
   int j;                     // entry_index
-  float v, x;                // its value and its logit
+  float v;                   // its value
+  T x;                       // its logit
 };
 
 template <typename T>
-__device__ __forceinline__ Entry load_entry(const Logits& p, const ListIn& q, unsigned r, int k, const T* x) {
-  Entry e{-1, 0.f, -INFINITY};
+__device__ __forceinline__ Entry<T> load_entry(const Logits& p, const ListIn& q, unsigned r, int k, const T* x) {
+  Entry<T> e{-1, 0.f, (T)0.f};
   if (k < q.k) {
     e.j = entry_index(q, (size_t)r * q.k + k, p.vocab);
     e.v = q.val[(size_t)r * q.k + k];
-    if (e.j >= 0) e.x = (float)x[e.j];
+    e.x = x[std::max(0, e.j)];
   }
   return e;
 }
 
 // A wave's part of the list: entry k of each lane (in `mine`), k + threads, ...  The whole wave calls it.
 template <typename T>
-__device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, unsigned r, const T* x, const Entry& mine, int k, int threads) {
+__device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, unsigned r, const T* x, const Entry<T>& mine, int k, int threads) {
   ListSum o;
   float m = -INFINITY, vref = -INFINITY;
   int used = 0, bad = 0;
-  Entry e = mine;
+  Entry<T> e = mine;
   for (int i = k;;) {
     bad |= e.j == -2;
     if (e.j >= 0) {
-      m = fmaxf(m, e.x);
+      m = fmaxf(m, (float)e.x);
       vref = fmaxf(vref, e.v == e.v ? e.v : INFINITY);
       ++used;
     }
@@ -90,12 +92,12 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
   e = mine;
   for (int i = k;;) {
     if (e.j >= 0) {
-      const float d = distance(e.x, ref, p.c), ex = __builtin_amdgcn_exp2f(d);
+      const float d = distance((float)e.x, ref, p.c), ex = __builtin_amdgcn_exp2f(d);
       const double lv = ((double)e.v - from) * it;
       const float ev = exp_wide(lv);
       s += ex;
       z += (double)ev;
-      if (ev != 0.f) gap += (double)ev * (lv - ((double)e.x - (double)ref.m) * p.inv_tau);
+      if (ev != 0.f) gap += (double)ev * (lv - ((double)(float)e.x - (double)ref.m) * p.inv_tau);
     }
     if ((i += threads) >= q.k) break;
     e = load_entry(p, q, r, i, x);
@@ -179,11 +181,11 @@ struct Unlisted {
 // each thread (in `mine`), t + threads, ...  x and out are the row's beginning.
 template <typename T>
 __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, unsigned r, const f32x4& a, const f32x4& b, float scale, int lo,
-                                           int n, const T* x, T* out, const Entry& mine, int t, int threads) {
+                                           int n, const T* x, T* out, const Entry<T>& mine, int t, int threads) {
   const float cv = q.tail ? (float)(1.0 / LN2) : p.c;
   const Ref ref = make_ref(a[2], p.c);
   const size_t first = (size_t)r * q.k;
-  Entry e = mine;
+  Entry<T> e = mine;
   for (int k = t;;) {
     if (e.j >= lo && e.j - lo < n) {
       float pk = 0.f;
@@ -193,7 +195,7 @@ __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, uns
       } else {
         pk = __builtin_amdgcn_exp2f((e.v - b[0]) * cv);
       }
-      const float ex = __builtin_amdgcn_exp2f(distance(e.x, ref, p.c));
+      const float ex = __builtin_amdgcn_exp2f(distance((float)e.x, ref, p.c));
       out[e.j] = (T)(scale * (a[3] * ex - b[1] * pk));
     }
     if ((k += threads) >= q.k) break;
@@ -279,7 +281,7 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
     return;
   }
   const T* x = reinterpret_cast<const T*>(p.x) + (counts ? row_offset(p, r) : 0);
-  Entry mine{-1, 0.f, -INFINITY};
+  Entry<T> mine{-1, 0.f, (T)0.f};
   if (counts) mine = load_entry(p, q, r, t, x);
   for (int i = t; i < words; i += TPR) marks.bits[i] = 0;
   Row<T, TPR, S::NCH> row;

@@ -370,8 +370,8 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
   row.load();
   // asked for before they are needed: they arrive with the row
   const bool inside = label >= 0 && label < p.vocab;
-  const float x_label = inside ? (float)x[label] : NAN, old = q.old_logp[r], ref = q.ref ? q.ref[r] : 0.f;
-  const float adv = q.adv[q.adv_per_sequence ? s : r];
+  const T x_label = x[inside ? label : 0];
+  const float old = q.old_logp[r], ref = q.ref ? q.ref[r] : 0.f, adv = q.adv[q.adv_per_sequence ? s : r];
   const double share = counted_share(u);
   const int own = q.per_sequence ? q.count[s] : 1;
   const Part m = row_join<TPR>(row.template stats<true>(p.c, Whole{}), p.c, red);
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
   if (TPR == 64 || threadIdx.x < 64) {
     const double w = one_over(share) / own;
     const RowStat st = finish(m, p);
-    const double logp = inside ? log_prob(x_label, st, p) : NAN;
+    const double logp = inside ? log_prob((float)x_label, st, p) : NAN;
     const TokenTerms k = token_terms(logp - (double)old, (double)ref - logp, q, (double)adv);
     if (st.inv_ts != 0.f) {
       const double a = q.scale * w * k.a, b = -q.scale * w * q.ent, over = (double)st.inv_ts;

@@ -412,10 +412,7 @@ struct Span {
 // TPR threads hold up to TPR * NCH vectors of a row in registers, so that its statistics and its gradient need one read of
 // memory; vectors beyond that (rows of more than 256 KB) are read again.  A wave passes over the vectors that none of its
 // lanes has.
-template <typename T> __device__ __forceinline__ u32x4 no_elements();       // -inf: adds nothing, changes no maximum
-template <> __device__ __forceinline__ u32x4 no_elements<float>() { return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }
-template <> __device__ __forceinline__ u32x4 no_elements<__bf16>() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
-template <> __device__ __forceinline__ u32x4 no_elements<_Float16>() { return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u}; }
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 struct Whole {                // nothing of a row is left out
   __device__ __forceinline__ void vector(int, int, float*) const {}
@@ -432,20 +429,34 @@ struct Row : Span<T, TPR> {
   using Base::t;
   using Base::x;
   u32x4 v[NCH];
-  float extra;                // the element outside the vectors, -inf without one
-  int slots;                  // vectors of v that any lane of the wave has
+  T outside;                  // the element outside the vectors
+  int slots, full;            // vectors of v that any lane of the wave has; that all its lanes have
 
   __device__ __forceinline__ void place(const T* row, int elements, int thread) { static_cast<Base&>(*this) = Base(row, elements, thread); }
 
+  // Buffer loads: one after the other without a branch between them, so that the first vector can be waited for alone; what
+  // lies behind the row is not asked for and comes back as 0.
   __device__ __forceinline__ void load() {
-    const int first = __builtin_amdgcn_readfirstlane(t);
-    slots = nv > first ? (nv - first + TPR - 1) / TPR : 0;
-    const u32x4* b = body();
+    outside = x[std::max(0, this->extra_at())];                // first, since loads return in order
+    const int first = scalar(t), last = nv - 1 - first;
+    slots = last < 0 ? 0 : last / TPR + 1;
+    full = last < 63 ? 0 : (last - 63) / TPR + 1;
+    const uint64_t at = reinterpret_cast<uint64_t>(body());
+    const uint64_t base = (uint64_t)(uint32_t)scalar((int)(at >> 32)) << 32 | (uint32_t)scalar((int)at);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, scalar(std::min(nv, NCH * TPR)) * 16, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
-      if (i < slots) v[i] = t + i * TPR < nv ? __builtin_nontemporal_load(b + t + i * TPR) : no_elements<T>();
-    const int at = this->extra_at();
-    extra = at >= 0 ? (float)x[at] : -INFINITY;
+    for (int i = 0; i < NCH; ++i) {
+      v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, t * 16 + i * TPR * 16, 0, 2));
+      __builtin_amdgcn_sched_barrier(0);                        // in this order
+    }
+  }
+  __device__ __forceinline__ float extra() const { return this->extra_at() >= 0 ? (float)outside : -INFINITY; }
+  // the elements of vector i; -inf where the lane has none
+  __device__ __forceinline__ void elements(int i, float* f) const {
+    Type<T>::unpack(v[i], f);
+    if (i >= full)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = t + i * TPR < nv ? f[j] : -INFINITY;
   }
 
   // Between two passes over the registers: what a pass made of them (twice as many floats of a 16-bit type) is made again
@@ -459,11 +470,11 @@ struct Row : Span<T, TPR> {
   // the thread's `slot`-th vector, and of the element outside the vectors.
   template <bool WANT_W, typename F>
   __device__ __forceinline__ Part stats(float c, const F& leave_out) {
-    const float outside = leave_out.extra(t, extra);
-    float g = outside;
+    const float beside = leave_out.extra(t, extra());
+    float g = beside;
     if (slots > 0) {
       float f[VEC];
-      Type<T>::unpack(v[0], f);
+      elements(0, f);
       leave_out.vector(0, t, f);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) g = fmaxf(g, f[j]);
@@ -472,7 +483,7 @@ struct Row : Span<T, TPR> {
     const Ref ref = make_ref(g, c);
     Part p{ref.m, 0.f, 0.f};
     if (!ref.low) {
-      add_up<1, false, WANT_W>(&outside, ref, c, p.s, p.w);
+      add_up<1, false, WANT_W>(&beside, ref, c, p.s, p.w);
 #pragma unroll
       for (int i = 0; i < NCH; i += 4) {
         float s = 0.f, w = 0.f;
@@ -480,7 +491,7 @@ struct Row : Span<T, TPR> {
         for (int k = 0; k < 4; ++k)
           if (i + k < slots) {
             float f[VEC];
-            Type<T>::unpack(v[i + k], f);
+            elements(i + k, f);
             leave_out.vector(i + k, t, f);
             add_up<VEC, false, WANT_W>(f, ref, c, s, w);
           }
@@ -491,7 +502,7 @@ struct Row : Span<T, TPR> {
     int from = NCH;
     if (ref.low || !__all(p.s < FAR)) {                         // another reference is needed: again, with the largest so far
       p = Part{-INFINITY, 0.f, 0.f};
-      take<1, WANT_W>(p, &outside, c);
+      take<1, WANT_W>(p, &beside, c);
       from = 0;
     }
     for (int slot = from; t + slot * TPR < nv; ++slot) {
