@@ -263,6 +263,24 @@ __device__ __forceinline__ void no_list(const ListIn& q, const Sums& u, unsigned
   if (t < 2 && q.row) q.row[2 * (size_t)r + t] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
+// LDS, and for its own stores memory, of a row's threads in order: they are a block, or a wave, whose accesses keep their
+// order by themselves.
+template <int TPR>
+__device__ __forceinline__ void sync_row() {
+  if (TPR > 64) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+template <int TPR>
+__device__ __forceinline__ bool sync_row_or(bool v) {
+  if (TPR > 64) return __syncthreads_or(v);
+  sync_row<TPR>();
+  return __any(v);
+}
+
 template <typename T, typename S>
 __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, Sums u, int words, T* __restrict__ grad) {
   constexpr int TPR = S::TPR, VEC = Type<T>::VEC;
@@ -275,20 +293,21 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   const M marks{all_bits + (threadIdx.x / TPR) * words};
   const unsigned r = blockIdx.x * S::ROWS + threadIdx.x / TPR;
   const bool counts = r < p.rows && (!q.mask || q.mask[r]);
-  if (S::ROWS == 1 && !counts) {                                // the whole block
+  if (!counts) {                                                // all threads of the row
+    if (r >= p.rows) return;
     no_list(q, u, r, t);
     if (grad) store_zeros<T, TPR>(grad + (size_t)r * p.vocab, p.vocab, t);
     return;
   }
-  const T* x = reinterpret_cast<const T*>(p.x) + (counts ? row_offset(p, r) : 0);
-  Entry<T> mine{-1, 0.f, (T)0.f};
-  if (counts) mine = load_entry(p, q, r, t, x);
+  const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r);
+  const Entry<T> mine = load_entry(p, q, r, t, x);
   for (int i = t; i < words; i += TPR) marks.bits[i] = 0;
   Row<T, TPR, S::NCH> row;
-  row.place(x, counts ? p.vocab : 0, t);
-  __syncthreads();
+  row.place(x, p.vocab, t);
+  sync_row<TPR>();
   bool twice = false;
-  if (counts && __builtin_amdgcn_readfirstlane(t) < q.k) {
+  const bool has_entries = scalar(t) < q.k;                     // of the wave
+  if (has_entries) {
     if (mine.j >= 0) twice = marks.set(row, mine.j, words - 1);
     for (int k = t + TPR; k < q.k; k += TPR) {
       const int j = entry_index(q, (size_t)r * q.k + k, p.vocab);
@@ -297,20 +316,13 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   }
   row.load();
   const double share = q.mask ? counted_share(u) : 0.0;
-  if (TPR == 64) {
-    __syncthreads();
-    twice = __any(twice);
-  } else {
-    twice = __syncthreads_or(twice);
-  }
+  twice = sync_row_or<TPR>(twice);
   ListSum list{0.0, 0.0, -INFINITY, 0.f, -INFINITY, 0, 0};
-  if (counts && __builtin_amdgcn_readfirstlane(t) < q.k) list = sum_list(p, q, r, x, mine, t, TPR);
+  if (has_entries) list = sum_list(p, q, r, x, mine, t, TPR);
   if (TPR > 64 && (threadIdx.x & 63) == 0) lists[threadIdx.x >> 6] = list;     // read behind row_join's barrier
   const Part m = row_join<TPR>(row.template stats<false>(p.c, Unlisted<M>{marks, words - 1}), p.c, red);
   f32x4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
-  if (!counts) {                                                // TPR = 64: a wave's row
-    if (r < p.rows) no_list(q, u, r, t);
-  } else if (TPR == 64 || threadIdx.x < 64) {
+  if (TPR == 64 || threadIdx.x < 64) {
     if (TPR > 64) list = join_lists(p, q, threadIdx.x < TPR / 64 ? lists[threadIdx.x] : ListSum{0.0, 0.0, -INFINITY, 0.f, -INFINITY, 0, 0});
     if (twice) list = without_repeats(p, q, r, x, list);
     const double w = q.mask ? one_over(share) : 1.0 / u.rows;
@@ -335,12 +347,13 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   }
   T* out = grad + (size_t)r * p.vocab;
   const bool zero = b[3] == 0.f;
-  if (r < p.rows) {
-    if (zero) store_zeros<T, TPR>(out, p.vocab, t);
-    else row.store(out, f32x4{a[0], a[1], 0.f, 0.f}, p.c, -1);
+  if (zero) {
+    store_zeros<T, TPR>(out, p.vocab, t);
+    return;
   }
-  __syncthreads();                                              // a listed element is written twice, in this order
-  if (!zero) patch_list<T>(p, q, r, a, b, 1.f, 0, p.vocab, x, out, mine, t, TPR);
+  row.store(out, f32x4{a[0], a[1], 0.f, 0.f}, p.c, -1);
+  sync_row<TPR>();                                              // a listed element is written twice, in this order
+  if (has_entries) patch_list<T>(p, q, r, a, b, 1.f, 0, p.vocab, x, out, mine, t, TPR);
 }
 
 // the gradient again, for another upstream gradient or a second time

@@ -369,6 +369,9 @@ __device__ __forceinline__ u32x4 gradient_vector(const u32x4& w, const f32x4& k,
 template <typename T, int TPR>
 struct Span {
   static constexpr int VEC = Type<T>::VEC;
+  // Loads in flight where a row is read again: four where rows are larger than their threads' registers, one where that
+  // happens to rare rows only (more would cost every row the registers).
+  static constexpr int AGAIN = TPR == 1024 ? 4 : 1;
   const T* x;
   int n, t, head, nv;
   __device__ __forceinline__ Span() {}
@@ -390,7 +393,14 @@ struct Span {
   template <bool BOTH, bool IS_LOW>
   __device__ __forceinline__ void stream(T* out, const f32x4& k, const Ref& ref, float c, int first) const {
     u32x4_u* o = reinterpret_cast<u32x4_u*>(out + head);
-    for (int i = t + first; i < nv; i += TPR) o[i] = gradient_vector<T, BOTH, IS_LOW>(body()[i], k, ref, c);
+    for (int i = t + first; i < nv; i += AGAIN * TPR) {
+      u32x4 b[AGAIN];
+#pragma unroll
+      for (int q = 0; q < AGAIN; ++q) b[q] = body()[std::min(i + q * TPR, nv - 1)];
+#pragma unroll
+      for (int q = 0; q < AGAIN; ++q)
+        if (i + q * TPR < nv) o[i + q * TPR] = gradient_vector<T, BOTH, IS_LOW>(b[q], k, ref, c);
+    }
     const int j = extra_at();
     if (j >= 0) out[j] = (T)gradient_entry<BOTH, IS_LOW>((float)x[j], k, ref, c);
   }
@@ -410,7 +420,7 @@ struct Span {
 
 // ---- a row held by its threads -------------------------------------------------------------------------------------------
 // TPR threads hold up to TPR * NCH vectors of a row in registers, so that its statistics and its gradient need one read of
-// memory; vectors beyond that (rows of more than 256 KB) are read again.  A wave passes over the vectors that none of its
+// memory; vectors beyond that (rows of more than 320 KB) are read again.  A wave passes over the vectors that none of its
 // lanes has.
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -422,6 +432,7 @@ struct Whole {                // nothing of a row is left out
 template <typename T, int TPR, int NCH>
 struct Row : Span<T, TPR> {
   using Base = Span<T, TPR>;
+  using Base::AGAIN;
   using Base::VEC;
   using Base::body;
   using Base::n;
@@ -505,11 +516,22 @@ struct Row : Span<T, TPR> {
       take<1, WANT_W>(p, &beside, c);
       from = 0;
     }
-    for (int slot = from; t + slot * TPR < nv; ++slot) {
-      float f[VEC];
-      Type<T>::unpack(body()[t + slot * TPR], f);
-      leave_out.vector(slot, t, f);
-      take<VEC, WANT_W>(p, f, c);
+    for (int slot = from; t + slot * TPR < nv; slot += AGAIN) {
+      u32x4 b[AGAIN];
+      float f[AGAIN * VEC];
+#pragma unroll
+      for (int k = 0; k < AGAIN; ++k) b[k] = body()[std::min(t + (slot + k) * TPR, nv - 1)];
+#pragma unroll
+      for (int k = 0; k < AGAIN; ++k) {
+        Type<T>::unpack(b[k], f + k * VEC);
+        if (t + (slot + k) * TPR < nv) {
+          leave_out.vector(slot + k, t, f + k * VEC);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) f[k * VEC + j] = -INFINITY;
+        }
+      }
+      take<AGAIN * VEC, WANT_W>(p, f, c);
     }
     return p;
   }
@@ -675,7 +697,7 @@ inline void launch_sum_terms(const Sums& q, hipStream_t s) {
 // Which of the row kernels takes a row of `bytes`: the fewest threads that hold it with 16 vectors each, so that as many
 // rows as possible share a compute unit, each in another phase of its work (16 vectors and about 50 more registers leave
 // room for 16 waves, 256 KB of rows); rows of up to 16 KB are a wave's and meet no barrier.  The largest reads again what is
-// beyond 256 KB.  `kernel` is called with the two numbers as a type.
+// beyond 320 KB.  `kernel` is called with the two numbers as a type.
 template <int A, int B> struct Shape {
   static constexpr int TPR = A, NCH = B, BLOCK = A == 64 ? 256 : A, ROWS = BLOCK / A;
 };
@@ -687,7 +709,8 @@ auto with_shape(long long bytes, F kernel) {
   if (bytes <= 32 << 10) return kernel(Shape<128, 16>{});
   if (bytes <= 64 << 10) return kernel(Shape<256, 16>{});
   if (bytes <= 128 << 10) return kernel(Shape<512, 16>{});
-  return kernel(Shape<1024, 16>{});
+  if (bytes <= 256 << 10) return kernel(Shape<1024, 16>{});
+  return kernel(Shape<1024, 20>{});                             // 320 KB of it
 }
 template <typename F>
 auto with_type(int dtype, F f) {
