@@ -47,33 +47,34 @@ class PolicyOutput(NamedTuple):
     stats: torch.Tensor                # means of the surrogate, the KL estimate, the entropy, "the clip holds the ratio"
 
 
-# ---- arguments ------------------------------------------------------------------------------------------------------------
+# ---- arguments (checked once a call: a small loss is bound by what happens here) ------------------------------------------------
 def _logits_args(x: torch.Tensor):
     """(x, dtype, rows, inner, s_outer, s_inner, vocab) of the C ABI."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("logits: expected a torch.Tensor")
-    if x.dtype not in _DTYPES:
+    code, shape = _DTYPES.get(x.dtype), x.shape
+    if code is None:
         raise _lib.StHipError(f"logits: expected fp32, bf16 or fp16, got {x.dtype}")
-    if x.dim() not in (2, 3) or x.shape[-1] == 0:
-        raise _lib.StHipError(f"logits: expected [T, V] or [B, L, V], got {tuple(x.shape)}")
+    if len(shape) not in (2, 3) or shape[-1] == 0:
+        raise _lib.StHipError(f"logits: expected [T, V] or [B, L, V], got {tuple(shape)}")
     if not x.is_cuda:
         raise _lib.StHipError(f"logits: the HIP hot path needs a tensor on the GPU, got device={x.device} (no CPU fallback)")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
-        raise _lib.StHipError(f"logits: the vocabulary's stride is {x.stride(-1)}, expected 1")
-    code, vocab = _DTYPES[x.dtype], x.shape[-1]
-    if x.dim() == 2:
-        return x.data_ptr(), code, x.shape[0], max(1, x.shape[0]), 0, x.stride(0), vocab
-    return x.data_ptr(), code, x.shape[0] * x.shape[1], max(1, x.shape[1]), x.stride(0), x.stride(1), vocab
+    stride = x.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
+        raise _lib.StHipError(f"logits: the vocabulary's stride is {stride[-1]}, expected 1")
+    if len(shape) == 2:
+        return x.data_ptr(), code, shape[0], shape[0] or 1, 0, stride[0], shape[1]
+    return x.data_ptr(), code, shape[0] * shape[1], shape[1] or 1, stride[0], stride[1], shape[2]
 
 
 def _whole(t: torch.Tensor, name: str, like: torch.Tensor, shape) -> torch.Tensor:
     """An index tensor beside the logits: int64 or int32, the shape asked for, contiguous."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
-    if t.dtype not in (torch.int64, torch.int32):
+    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
         raise _lib.StHipError(f"{name}: expected int64 or int32, got {t.dtype}")
     _beside(t, name, like, shape)
-    return t.detach().contiguous()
+    return t.contiguous()
 
 
 def _floats(t: torch.Tensor, name: str, like: torch.Tensor, shape) -> torch.Tensor:
@@ -89,12 +90,12 @@ def _floats(t: torch.Tensor, name: str, like: torch.Tensor, shape) -> torch.Tens
 def _beside(t, name, like, shape):
     if t.device != like.device:
         raise _lib.StHipError(f"{name}: on {t.device}, the logits are on {like.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise _lib.StHipError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _label_args(labels: torch.Tensor, ignore_index: int):
-    return labels.data_ptr(), int(labels.dtype == torch.int64), ignore_index
+    return labels.data_ptr(), int(labels.dtype is torch.int64), ignore_index
 
 
 def _ignore(ignore_index) -> int:
@@ -125,19 +126,30 @@ def _sequences(x: torch.Tensor, cu_seqlens: Optional[torch.Tensor]):
     return cu.numel() - 1, cu
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(x: torch.Tensor):
     """The logits' device as the current one while a kernel is enqueued on its current stream."""
     if x.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(x.device)
 
 
-def _buffer(x: torch.Tensor, nbytes: int) -> torch.Tensor:
-    return torch.empty(max(16, nbytes), dtype=torch.uint8, device=x.device)
-
-
 def _f32(x: torch.Tensor, *shape) -> torch.Tensor:
-    return torch.empty(shape, dtype=torch.float32, device=x.device)
+    return x.new_empty(shape, dtype=torch.float32)
+
+
+def _scratch(x: torch.Tensor, kept: int, work: int):
+    """(buffer, address of its first ``kept`` bytes, which a backward pass reads, address of the workspace behind them)."""
+    kept = -(-kept // 256) * 256
+    buffer = x.new_empty((kept + work + 16,), dtype=torch.uint8)
+    at = buffer.data_ptr()
+    return buffer, at, at + kept
+
+
+def _grad_buffer(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -149,104 +161,98 @@ def _gout(g: torch.Tensor) -> torch.Tensor:
 
 
 # ---- log-probabilities ------------------------------------------------------------------------------------------------------
-def _logprobs_fwd(x, labels, tau, ignore, want_entropy, want_state):
+def _logprobs_fwd(x, args, labels, tau, ignore, want_entropy, want_state):
     lib = _lib.load()
-    args = _logits_args(x)
-    shape = x.shape[:-1]
+    shape = labels.shape
     logp = _f32(x, *shape)
     entropy = _f32(x, *shape) if want_entropy else None
-    state = _f32(x, *shape, 4) if want_state else None
     with _on(x):
-        work = _buffer(x, lib.st_token_workspace_bytes(args[1], args[2], args[6], 0))
-        _lib.check(lib.st_token_logprobs_fwd(*args, *_label_args(labels, ignore), tau, logp.data_ptr(), _ptr(entropy), _ptr(state),
-                                             work.data_ptr(), _lib.stream_ptr()), "st_token_logprobs_fwd")
-    return logp, entropy, state
+        buffer, state, work = _scratch(x, 16 * args[2] if want_state else 0, lib.st_token_workspace_bytes(args[1], args[2], args[6], 0))
+        _lib.check(lib.st_token_logprobs_fwd(*args, *_label_args(labels, ignore), tau, logp.data_ptr(), _ptr(entropy),
+                                             state if want_state else None, work, _lib.stream_ptr()), "st_token_logprobs_fwd")
+    return logp, entropy, buffer
 
 
 class _TokenLogProbsFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, labels, tau, ignore, want_entropy):
-        logp, entropy, state = _logprobs_fwd(x, labels, tau, ignore, want_entropy, True)
-        ctx.tau, ctx.ignore = tau, ignore
+    def forward(ctx, x, call):
+        args, labels, tau, ignore, want_entropy = call
+        logp, entropy, buffer = _logprobs_fwd(x, args, labels, tau, ignore, want_entropy, True)
+        ctx.call = args, tau, ignore
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, labels, state)
+        ctx.save_for_backward(x, labels, buffer)
         return (logp, entropy) if want_entropy else logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logp, g_entropy=None):
         if g_logp is None and g_entropy is None:
-            return None, None, None, None, None
+            return None, None
         x, labels, state = ctx.saved_tensors
-        lib = _lib.load()
+        args, tau, ignore = ctx.call
         grad = _grad_buffer(x)
         g_logp = None if g_logp is None else _gout(g_logp)
         g_entropy = None if g_entropy is None else _gout(g_entropy)
         with _on(x):
-            _lib.check(lib.st_token_logprobs_bwd(*_logits_args(x), *_label_args(labels, ctx.ignore), ctx.tau, state.data_ptr(),
-                                                 _ptr(g_logp), _ptr(g_entropy), grad.data_ptr(), _lib.stream_ptr()),
-                       "st_token_logprobs_bwd")
-        return grad, None, None, None, None
+            _lib.check(_lib.load().st_token_logprobs_bwd(*args, *_label_args(labels, ignore), tau, state.data_ptr(), _ptr(g_logp), _ptr(g_entropy),
+                                                         grad.data_ptr(), _lib.stream_ptr()), "st_token_logprobs_bwd")
+        return grad, None
 
 
 def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: float = 1.0, ignore_index: int = -100,
                    return_entropy: bool = False):
     """``log softmax(logits / temperature)`` at each position's label, fp32 of the labels' shape; with ``return_entropy``
     also the entropy of each position's distribution.  Both are differentiable."""
-    _logits_args(logits)
+    args = _logits_args(logits)
     labels = _whole(labels, "labels", logits, logits.shape[:-1])
     tau, ignore = _temperature(temperature), _ignore(ignore_index)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _TokenLogProbsFunction.apply(logits, labels, tau, ignore, bool(return_entropy))
-    logp, entropy, _ = _logprobs_fwd(logits, labels, tau, ignore, return_entropy, False)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TokenLogProbsFunction.apply(logits, (args, labels, tau, ignore, bool(return_entropy)))
+    logp, entropy, _ = _logprobs_fwd(logits, args, labels, tau, ignore, return_entropy, False)
     return (logp, entropy) if return_entropy else logp
 
 
 # ---- the two losses whose rows go through the label's log-probability -------------------------------------------------------------
-def _grad_buffer(x: torch.Tensor) -> torch.Tensor:
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-
-
 def _take_grad(ctx, x):
     """(buffer, 1) the first time: it holds the gradient for an upstream gradient of 1, written by the forward kernel while the
     rows were on chip.  The buffer is given away, so a second backward pass gets a new one, (buffer, 0)."""
-    grad, ctx.grad = getattr(ctx, "grad", None), None
+    grad, ctx.grad = ctx.grad, None
     return (_grad_buffer(x), 0) if grad is None else (grad, 1)
 
 
-def _token_loss_bwd(ctx, x, labels, row_grad, gout):
-    lib = _lib.load()
+def _token_loss_bwd(ctx, gout):
+    x, labels, row_grad = ctx.saved_tensors
+    args, tau, ignore = ctx.call
     grad, for_one = _take_grad(ctx, x)
     gout = _gout(gout)
     with _on(x):
-        _lib.check(lib.st_token_loss_bwd(*_logits_args(x), *_label_args(labels, ctx.ignore), ctx.tau, row_grad.data_ptr(), gout.data_ptr(),
-                                         for_one, grad.data_ptr(), _lib.stream_ptr()), "st_token_loss_bwd")
-    return grad
+        _lib.check(_lib.load().st_token_loss_bwd(*args, *_label_args(labels, ignore), tau, row_grad.data_ptr(), gout.data_ptr(), for_one,
+                                                 grad.data_ptr(), _lib.stream_ptr()), "st_token_loss_bwd")
+    return grad, None
 
 
 class _PreferenceFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, labels, cu, ref, pairs, ignore, kind, average, beta, smoothing, scale):
+    def forward(ctx, x, call):
+        args, labels, ignore, cu, pairs, ref, kind, average, beta, smoothing, scale = call
         lib = _lib.load()
-        args = _logits_args(x)
         rows, need = args[2], ctx.needs_input_grad[0]
         loss, rewards = _f32(x), _f32(x, 2 * pairs)
-        row_grad = _f32(x, rows, 4) if need else None
         with _on(x):
-            work = _buffer(x, lib.st_token_workspace_bytes(args[1], rows, args[6], 2 * pairs))
+            buffer, row_grad, work = _scratch(x, 16 * rows if need else 0, lib.st_token_workspace_bytes(args[1], rows, args[6], 2 * pairs))
             _lib.check(lib.st_preference_loss_fwd(*args, *_label_args(labels, ignore), _ptr(cu), pairs, _ptr(ref), kind, average, beta, smoothing,
-                                                  scale, loss.data_ptr(), rewards.data_ptr(), _ptr(row_grad), work.data_ptr(),
+                                                  scale, loss.data_ptr(), rewards.data_ptr(), row_grad if need else None, work,
                                                   _lib.stream_ptr()), "st_preference_loss_fwd")
         ctx.mark_non_differentiable(rewards)
-        ctx.tau, ctx.ignore = 1.0, ignore
         if need:
-            ctx.save_for_backward(x, labels, row_grad)
+            ctx.call, ctx.grad = (args, 1.0, ignore), None
+            ctx.save_for_backward(x, labels, buffer)
         return loss, rewards
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout, _rewards):
-        return (_token_loss_bwd(ctx, *ctx.saved_tensors, gout), *(None,) * 10)
+        return _token_loss_bwd(ctx, gout)
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: Optional[torch.Tensor] = None, *,
@@ -260,33 +266,29 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: Optio
     ``"ipo"``: ``(h - 1 / (2 beta))^2``; ``"hinge"``: ``max(0, 1 - beta h)``.
 
     Returns ``(loss, chosen_rewards, rejected_rewards)``; the rewards ``beta (L - ref_logps)`` are constants."""
-    _logits_args(logits)
+    args = _logits_args(logits)
     labels = _whole(labels, "labels", logits, logits.shape[:-1])
     sequences, cu = _sequences(logits, cu_seqlens)
     if sequences % 2:
         raise _lib.StHipError(f"preference_loss: {sequences} sequences: expected the chosen ones and as many rejected ones behind them")
     if kind not in _KINDS:
         raise _lib.StHipError(f"preference_loss: kind {kind!r}: expected one of {sorted(_KINDS)}")
-    beta, label_smoothing = float(beta), float(label_smoothing)
+    beta, label_smoothing, ignore = float(beta), float(label_smoothing), _ignore(ignore_index)
     if not 0.0 < beta < float("inf") or not 0.0 <= label_smoothing < 0.5:
         raise _lib.StHipError(f"preference_loss: beta={beta} label_smoothing={label_smoothing}: expected beta > 0 and 0 <= label_smoothing < 0.5")
     if label_smoothing and kind != "sigmoid":
         raise _lib.StHipError('preference_loss: label_smoothing goes with kind="sigmoid"')
     ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", logits, (sequences,))
     pairs = sequences // 2
-    if labels.numel() == 0 and pairs:
-        labels, logits, cu = labels.new_full((1,), int(ignore_index)), _no_row(logits), labels.new_zeros(sequences + 1, dtype=torch.int32)
     if pairs == 0:
-        return PreferenceOutput(_no_loss(logits), *(_f32(logits, 0) for _ in range(2)))
-    loss, rewards = _PreferenceFunction.apply(logits, labels, cu, ref, pairs, _ignore(ignore_index), _KINDS[kind], int(bool(average)), beta,
-                                              label_smoothing, float(scale))
+        return PreferenceOutput(_no_loss(logits), _f32(logits, 0), _f32(logits, 0))
+    if labels.numel() == 0:                                    # the references alone: one row that does not count, all sequences empty
+        labels, cu = labels.new_full((1,), ignore), labels.new_zeros(sequences + 1, dtype=torch.int32)
+        logits = torch.cat([logits.reshape(0, logits.shape[-1]), logits.new_zeros(1, logits.shape[-1])])
+        args = _logits_args(logits)
+    loss, rewards = _PreferenceFunction.apply(logits, (args, labels, ignore, cu, pairs, ref, _KINDS[kind], int(bool(average)), beta,
+                                                       label_smoothing, float(scale)))
     return PreferenceOutput(loss, rewards[:pairs], rewards[pairs:])
-
-
-def _no_row(logits: torch.Tensor) -> torch.Tensor:
-    """One row that does not count, for logits that have none; the gradient still reaches them."""
-    flat = logits.reshape(0, logits.shape[-1])
-    return torch.cat([flat, torch.zeros(1, logits.shape[-1], dtype=logits.dtype, device=logits.device)])
 
 
 def _no_loss(logits: torch.Tensor) -> torch.Tensor:
@@ -296,29 +298,28 @@ def _no_loss(logits: torch.Tensor) -> torch.Tensor:
 
 class _PolicyFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, labels, cu, old, adv, ref, sequences, tau, ignore, low, high, kl, ent, per_sequence, scale):
+    def forward(ctx, x, call):
+        args, labels, ignore, tau, cu, sequences, old, adv, ref, low, high, kl, ent, per_sequence, scale = call
         lib = _lib.load()
-        args = _logits_args(x)
         rows, need = args[2], ctx.needs_input_grad[0]
         loss, stats = _f32(x), _f32(x, 4)
-        row_grad = _f32(x, rows, 4) if need else None
         grad = _grad_buffer(x) if need else None
         with _on(x):
-            work = _buffer(x, lib.st_token_workspace_bytes(args[1], rows, args[6], sequences))
+            buffer, row_grad, work = _scratch(x, 16 * rows if need else 0, lib.st_token_workspace_bytes(args[1], rows, args[6], sequences))
             _lib.check(lib.st_policy_loss_fwd(*args, *_label_args(labels, ignore), tau, _ptr(cu), sequences, old.data_ptr(), adv.data_ptr(),
                                               int(adv.shape != labels.shape), _ptr(ref), low, high, kl, ent, per_sequence, scale,
-                                              loss.data_ptr(), stats.data_ptr(), _ptr(row_grad), _ptr(grad), work.data_ptr(),
+                                              loss.data_ptr(), stats.data_ptr(), row_grad if need else None, _ptr(grad), work,
                                               _lib.stream_ptr()), "st_policy_loss_fwd")
         ctx.mark_non_differentiable(stats)
-        ctx.tau, ctx.ignore, ctx.grad = tau, ignore, grad
         if need:
-            ctx.save_for_backward(x, labels, row_grad)
+            ctx.call, ctx.grad = (args, tau, ignore), grad
+            ctx.save_for_backward(x, labels, buffer)
         return loss, stats
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout, _stats):
-        return (_token_loss_bwd(ctx, *ctx.saved_tensors, gout), *(None,) * 14)
+        return _token_loss_bwd(ctx, gout)
 
 
 def clipped_policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
@@ -326,7 +327,7 @@ def clipped_policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: t
                         clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
                         reduction: str = "token", ignore_index: int = -100, scale: float = 1.0) -> PolicyOutput:
     """Clipped policy loss of sampled tokens.  With ``logp`` the label's log-probability, ``r = exp(logp - old_logps)`` and ``A``
-    the advantage (of each position, or ``[sequences]``: one for all of a sequence), a position's loss is
+    the advantage (the labels' shape: of each position; else ``[sequences]``: one for all of a sequence), a position's loss is
 
     ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - logp) - (ref - logp) - 1) - entropy_coef H``
 
@@ -336,7 +337,7 @@ def clipped_policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: t
 
     Returns ``(loss, stats)``: ``stats`` holds the same means of the surrogate, the KL estimate, the entropy and of whether the
     clip holds the ratio, as constants."""
-    _logits_args(logits)
+    args = _logits_args(logits)
     shape = logits.shape[:-1]
     labels = _whole(labels, "labels", logits, shape)
     sequences, cu = _sequences(logits, cu_seqlens)
@@ -354,42 +355,41 @@ def clipped_policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: t
     tau, ignore = _temperature(temperature), _ignore(ignore_index)
     if labels.numel() == 0:
         return PolicyOutput(_no_loss(logits), torch.zeros(4, device=logits.device))
-    return PolicyOutput(*_PolicyFunction.apply(logits, labels, cu, old, adv, ref, sequences, tau, ignore, clip_low, clip_high, kl_coef,
-                                               entropy_coef, _REDUCTIONS[reduction], float(scale)))
+    return PolicyOutput(*_PolicyFunction.apply(logits, (args, labels, ignore, tau, cu, sequences, old, adv, ref, clip_low, clip_high, kl_coef,
+                                                        entropy_coef, _REDUCTIONS[reduction], float(scale))))
 
 
 # ---- distillation -------------------------------------------------------------------------------------------------------------
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, idx, val, mask, tau, tail, scale):
+    def forward(ctx, x, call):
+        args, idx, val, mask, tau, tail, scale = call
         lib = _lib.load()
-        args = _logits_args(x)
         rows, need = args[2], ctx.needs_input_grad[0]
         loss = _f32(x)
-        row_grad = _f32(x, rows, 8) if need else None
         grad = _grad_buffer(x) if need else None
-        entries = (idx.data_ptr(), int(idx.dtype == torch.int64), val.data_ptr(), idx.shape[-1])
+        entries = (idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1])
         with _on(x):
-            work = _buffer(x, lib.st_distill_workspace_bytes(rows))
-            _lib.check(lib.st_distill_loss_fwd(*args, *entries, _ptr(mask), tau, tail, scale, loss.data_ptr(), _ptr(row_grad), _ptr(grad),
-                                               work.data_ptr(), _lib.stream_ptr()), "st_distill_loss_fwd")
-        ctx.tau, ctx.tail, ctx.grad = tau, tail, grad
+            buffer, row_grad, work = _scratch(x, 32 * rows if need else 0, lib.st_distill_workspace_bytes(rows))
+            _lib.check(lib.st_distill_loss_fwd(*args, *entries, _ptr(mask), tau, tail, scale, loss.data_ptr(), row_grad if need else None,
+                                               _ptr(grad), work, _lib.stream_ptr()), "st_distill_loss_fwd")
         if need:
-            ctx.save_for_backward(x, idx, val, row_grad)
+            ctx.call, ctx.grad = (args, tau, tail), grad
+            ctx.save_for_backward(x, idx, val, buffer)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
         x, idx, val, row_grad = ctx.saved_tensors
-        lib = _lib.load()
+        args, tau, tail = ctx.call
         grad, for_one = _take_grad(ctx, x)
         gout = _gout(gout)
         with _on(x):
-            _lib.check(lib.st_distill_loss_bwd(*_logits_args(x), idx.data_ptr(), int(idx.dtype == torch.int64), val.data_ptr(), idx.shape[-1],
-                                               ctx.tau, ctx.tail, row_grad.data_ptr(), gout.data_ptr(), for_one, grad.data_ptr(),
-                                               _lib.stream_ptr()), "st_distill_loss_bwd")
-        return grad, None, None, None, None, None, None
+            _lib.check(_lib.load().st_distill_loss_bwd(*args, idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1], tau, tail,
+                                                       row_grad.data_ptr(), gout.data_ptr(), for_one, grad.data_ptr(), _lib.stream_ptr()),
+                       "st_distill_loss_bwd")
+        return grad, None
 
 
 def topk_distill_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_values: torch.Tensor,
@@ -404,8 +404,9 @@ def topk_distill_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     they are the teacher's log-probabilities (at ``temperature``, over its whole vocabulary), and all tokens that are not listed
     form one more entry of the sum, with ``1 - sum_k p_k`` and the student's probability of the same tokens.
 
-    At most 2^20 tokens.  A position with no used entry contributes 0.  An index of ``V`` or more makes its position's loss and gradient NaN."""
-    _logits_args(logits)
+    At most 2^20 tokens.  A position with no used entry contributes 0.  An index of ``V`` or more makes its position's loss and
+    gradient NaN."""
+    args = _logits_args(logits)
     shape = logits.shape[:-1]
     if not isinstance(teacher_indices, torch.Tensor) or teacher_indices.dim() != logits.dim() or teacher_indices.shape[-1] == 0:
         raise _lib.StHipError("teacher_indices: expected [..., K] with K > 0 and the logits' leading shape")
@@ -413,14 +414,14 @@ def topk_distill_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     idx = _whole(teacher_indices, "teacher_indices", logits, entries)
     val = _floats(teacher_values, "teacher_values", logits, entries)
     if mask is not None:
-        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool:
+        if not isinstance(mask, torch.Tensor) or mask.dtype is not torch.bool:
             raise _lib.StHipError("mask: expected a bool tensor")
         _beside(mask, "mask", logits, shape)
-        mask = mask.detach().contiguous()
+        mask = mask.contiguous()
     tau = _temperature(temperature)
     if idx.numel() == 0:
         return _no_loss(logits)
-    return _DistillFunction.apply(logits, idx, val, mask, tau, int(bool(tail)), float(scale))
+    return _DistillFunction.apply(logits, (args, idx, val, mask, tau, int(bool(tail)), float(scale)))
 
 
 # ---- modules ------------------------------------------------------------------------------------------------------------------
