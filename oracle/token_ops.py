@@ -136,8 +136,8 @@ def distill(x, idx, val, mask=None, tau=1.0, tail=False):
             log_p = [(v - top) / tau - z if top > -math.inf else -math.inf for _, v in used]
         p = [math.exp(v) for v in log_p]
         each = sum(pk * (lk - float(log_q[j])) for pk, lk, (j, _) in zip(p, log_p, used) if pk > 0)
-        listed = sorted({j for j, _ in used})
-        off = [j for j in range(vocab) if j not in set(listed)]
+        listed = {j for j, _ in used}
+        off = [j for j in range(vocab) if j not in listed]
         mass = sum(p)
         rest = max(0.0, 1 - mass) if tail and off else 0.0
         g = q * (mass + rest)

@@ -19,8 +19,10 @@ pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
-#: half a step relative to the value, half the smallest step of a subnormal
-HALF = {torch.float32: (2.0 ** -24, 2.0 ** -150), torch.bfloat16: (2.0 ** -8, 2.0 ** -134), torch.float16: (2.0 ** -11, 2.0 ** -25)}
+#: Half a step relative to the value, and what is lost near 0: half the smallest step of fp16's subnormals; for the types with
+#: fp32's range, the exponential itself, whose result is 0 below the smallest normal number 2^-126 (times coefficients of at
+#: most 1, so an entry below it is off by at most that).
+HALF = {torch.float32: (2.0 ** -24, 2.0 ** -126), torch.bfloat16: (2.0 ** -8, 2.0 ** -126), torch.float16: (2.0 ** -11, 2.0 ** -25)}
 
 
 def row_error(vocab):
@@ -451,6 +453,96 @@ def test_distill_keeps_what_little_the_rest_holds():
     got.backward()
     assert abs(float(got.detach()) - loss) <= 1e-6 * loss
     close(leaf.grad, want, 1e-5 * want.abs(), "gradient")
+
+
+# ---- every size of row, and rows whose logits are far apart ------------------------------------------------------------------------
+#: sizes on both sides of every change of kernel: a wave's rows (4, 8, 16 KB), a block's (32, 64, 128, 256, 320 KB), and beyond
+SIZES = [(torch.bfloat16, v) for v in (2040, 2056, 4090, 8191, 8200, 16380, 16390, 32770, 65536, 65550, 131072, 131080, 170001)] + [
+    (torch.float32, v) for v in (1023, 1029, 2050, 4095, 8190, 16387, 32769, 65537, 81930, 131072)] + [(torch.float16, 20001), (torch.float16, 140001)]
+
+
+def far_logits(n, vocab, dtype, seed):
+    """Rows whose first vectors say nothing about the rest: masked, tiny, or far below what follows."""
+    x = logits(n, vocab, dtype, seed)
+    x[1, : vocab // 2] = -math.inf
+    x[2] = (x[2].float() * 4 - 60).to(dtype)
+    x[2, vocab - 2] = 60.0                                      # 170 bits above the first vectors
+    x[3, : vocab - vocab // 3] = torch.finfo(dtype).min
+    x[3, vocab // 2] = -3.0
+    return x
+
+
+@pytest.mark.parametrize("dtype,vocab", SIZES)
+def test_policy_rows_of_every_size(dtype, vocab):
+    from style_transfer_amd.losses import clipped_policy_loss
+    n, tau, ent, kl = 5, 1.1, 0.01, 0.1
+    x = far_logits(n, vocab, dtype, vocab)
+    t = torch.tensor([[vocab - 1, vocab - 2, vocab - 2, vocab // 2, -100]])
+    flat = t.view(-1)
+    logp, h, log_q, q = O.token_logprobs(x, flat, tau)
+    step = torch.tensor([0.1, -0.1, 0.5, 0.05, 0.0])
+    old, ref, adv = logp.float() + step, logp.float() - 0.25, torch.tensor([1.0, -1.0, 0.5, 2.0, 9.0])
+    loss, stats, want = O.policy(x, flat, [(0, n)], old, adv, ref, 0.2, 0.2, kl, ent, tau)
+    leaf = x.view(1, n, vocab).cuda().requires_grad_(True)
+    got = clipped_policy_loss(leaf, t.cuda(), old.view(1, n).cuda(), adv.view(1, n).cuda(), ref.view(1, n).cuda(), kl_coef=kl, entropy_coef=ent,
+                              temperature=tau)
+    got.loss.backward()
+    # old and ref are as far from 0 as the log-probabilities: 2 U of them comes on top of a row's error
+    err = row_error(vocab) + 40 * U + 2 * U * float(logp.abs().max())
+    close(got.stats, stats, torch.tensor([4 * err, 4 * err, 14 * err, 2 * U]) + stats.abs() * 2 * U, "stats")
+    close(got.loss, torch.tensor(loss), 5 * err + 4 * U * float(stats.abs().sum()), "loss")
+    w = torch.tensor([0.25] * 4 + [0.0], dtype=torch.float64)
+    close(leaf.grad[0], want, grad_bound(want, dtype, log_q, w * (2 * adv.double().abs() + 4 * kl), w * ent, h, tau, extra=err), "gradient")
+    with torch.no_grad():
+        again = clipped_policy_loss(leaf, t.cuda(), old.view(1, n).cuda(), adv.view(1, n).cuda(), ref.view(1, n).cuda(), kl_coef=kl,
+                                    entropy_coef=ent, temperature=tau)
+    assert torch.equal(again.loss, got.loss.detach()) and torch.equal(again.stats, got.stats)
+
+
+@pytest.mark.parametrize("dtype,vocab", SIZES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_rows_of_every_size(dtype, vocab, tail):
+    from style_transfer_amd.losses import topk_distill_loss
+    n, k, tau = 5, 70, 1.3
+    x = far_logits(n, vocab, dtype, vocab + 1)
+    idx, val = teacher(torch.zeros(n, vocab), k, tau, tail, vocab)
+    idx[:, 0], idx[:, 1], idx[:, 2] = vocab - 1, vocab // 2, 0  # the last element, a finite one of the masked row, the first
+    idx[:, 3:] = torch.where((idx[:, 3:] == vocab - 1) | (idx[:, 3:] == vocab // 2) | (idx[:, 3:] == 0), -1, idx[:, 3:])
+    masked = x.gather(1, idx.clamp(min=0).long()) <= torch.finfo(dtype).min
+    val = val.masked_fill(masked, -math.inf)                    # the teacher has no mass where the student is masked
+    mask = torch.tensor([True, True, True, True, False])
+    loss, want = O.distill(x, idx, val, mask, tau, tail)
+    leaf = x.cuda().requires_grad_(True)
+    got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), mask.cuda(), temperature=tau, tail=tail)
+    got.backward()
+    # a term p (log p - log q) is off by a row's error and by 8 U of log q, which reaches 250 here
+    close(got, torch.tensor(loss), tau * tau * (2 * row_error(vocab) + 60 * U) + abs(loss) * 8 * U, "loss")
+    close(leaf.grad, want, distill_bound(x, idx, val, mask, tau, want, dtype), "gradient")
+
+
+def test_a_padded_batch_in_place():
+    """Rows of a slice at every alignment through the kernels that hold a row: as of a copy, and no other memory is written."""
+    from style_transfer_amd import losses
+    vocab = 2500
+    base = logits(2 * 5, vocab + 9, torch.bfloat16, 2).view(2, 5, vocab + 9).cuda()
+    t = labels_for(2 * 3, vocab, 4).view(2, 3).cuda()
+    idx, val = teacher(torch.zeros(6, vocab), 9, 1.0, True, 3)
+    idx, val, old = idx.view(2, 3, 9).cuda(), val.view(2, 3, 9).cuda(), torch.full((2, 3), -8.0).cuda()
+    for off in range(9):
+        for fn in (lambda v: losses.clipped_policy_loss(v, t, old, old[:, 0] + 9).loss, lambda v: losses.topk_distill_loss(v, idx, val, tail=True),
+                   lambda v: losses.preference_loss(v, t).loss):
+            leaf = base.clone().requires_grad_(True)
+            view = leaf[:, 1:4, off:off + vocab]
+            copy = view.detach().contiguous().requires_grad_(True)
+            a, b = fn(view), fn(copy)
+            a.backward()
+            b.backward()
+            assert abs(float(a.detach()) - float(b.detach())) <= 4 * row_error(vocab) * (1 + abs(float(b.detach())))
+            inner = leaf.grad[:, 1:4, off:off + vocab].float()
+            assert torch.allclose(inner, copy.grad.float(), atol=4 * row_error(vocab), rtol=2 * 2.0 ** -8)
+            outer = leaf.grad.clone()
+            outer[:, 1:4, off:off + vocab] = 0
+            assert not outer.any()
 
 
 # ---- how they are used --------------------------------------------------------------------------------------------------------
