@@ -23,7 +23,7 @@ __device__ __forceinline__ float load_one(const void* base, long long i) {
 template <typename T>
 __device__ __forceinline__ void write_row(const Logits& p, unsigned r, long long label, const Part& q, float* logp, float* entropy,
                                           f32x4* state) {
-  const RowStat st = finish(q, p);
+  const RowStat st = finish<true>(q, p);
   float lp = NAN, h = st.h, inv = st.inv_ts;
   if (label >= 0 && label < p.vocab) lp = (float)log_prob(load_one<T>(p.x, row_offset(p, r) + label), st, p);
   else inv = NAN;                                              // a label outside the vocabulary: visible, never an access
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, 
   f32x4 g{0.f, 0.f, 0.f, 0.f};
   if (TPR == 64 || threadIdx.x < 64) {
     const double w = one_over(share) / own;
-    const RowStat st = finish(m, p);
+    const RowStat st = finish<false>(m, p);
     const double logp = inside ? log_prob((float)x_label, st, p) : NAN;
     const TokenTerms k = token_terms(logp - (double)old, (double)ref - logp, q, (double)adv);
     if (st.inv_ts != 0.f) {

@@ -293,13 +293,16 @@ __device__ __forceinline__ float reciprocal(float v) {
 // what a reference is in x / tau: m c is rounded, and stands for itself
 __device__ __forceinline__ double logit_of(const Ref& r, const Logits& p) { return r.low ? (double)r.m * p.inv_tau : (double)r.mc * p.inv_ct; }
 
+// SUMMED: log-probabilities that a caller adds up over hundreds of tokens, where a mean error counts: ln_wide's is 2e-8, the
+// fp64 logarithm leaves the exponentials' 1e-8.
+template <bool SUMMED>
 __device__ __forceinline__ RowStat finish(const Part& q, const Logits& p) {
   RowStat r;
   const Ref ref = make_ref(q.m, p.c);
   const float inv = reciprocal(q.s);
   r.ref = ref.m;
   r.z = logit_of(ref, p);
-  r.ln_s = ln_wide(fmaf(-p.eps_ln2, q.w, q.s));
+  r.ln_s = SUMMED ? log((double)q.s - (double)p.eps_ln2 * (double)q.w) : ln_wide(fmaf(-p.eps_ln2, q.w, q.s));
   r.h = (float)(r.ln_s - p.inv_ct * (double)q.w * (double)inv);
   r.inv_ts = (float)(p.inv_tau * (double)inv);
   if (q.s == 0.f) {
