@@ -206,10 +206,14 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
     args = _logits_args(logits)
     labels = _whole(labels, "labels", logits, logits.shape[:-1])
     tau, ignore = _temperature(temperature), _ignore(ignore_index)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _wants_grad(logits):
         return _TokenLogProbsFunction.apply(logits, (args, labels, tau, ignore, bool(return_entropy)))
     logp, entropy, _ = _logprobs_fwd(logits, args, labels, tau, ignore, return_entropy, False)
     return (logp, entropy) if return_entropy else logp
+
+
+def _wants_grad(x: torch.Tensor) -> bool:
+    return x.requires_grad and torch.is_grad_enabled()
 
 
 # ---- the two losses whose rows go through the label's log-probability -------------------------------------------------------------
@@ -231,22 +235,26 @@ def _token_loss_bwd(ctx, gout):
     return grad, None
 
 
+def _preference_fwd(x, call, need):
+    args, labels, ignore, cu, pairs, ref, kind, average, beta, smoothing, scale = call
+    lib = _lib.load()
+    rows = args[2]
+    loss, rewards = _f32(x), _f32(x, 2 * pairs)
+    with _on(x):
+        buffer, row_grad, work = _scratch(x, 16 * rows if need else 0, lib.st_token_workspace_bytes(args[1], rows, args[6], 2 * pairs))
+        _lib.check(lib.st_preference_loss_fwd(*args, *_label_args(labels, ignore), _ptr(cu), pairs, _ptr(ref), kind, average, beta, smoothing,
+                                              scale, loss.data_ptr(), rewards.data_ptr(), row_grad if need else None, work,
+                                              _lib.stream_ptr()), "st_preference_loss_fwd")
+    return loss, rewards, buffer
+
+
 class _PreferenceFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        args, labels, ignore, cu, pairs, ref, kind, average, beta, smoothing, scale = call
-        lib = _lib.load()
-        rows, need = args[2], ctx.needs_input_grad[0]
-        loss, rewards = _f32(x), _f32(x, 2 * pairs)
-        with _on(x):
-            buffer, row_grad, work = _scratch(x, 16 * rows if need else 0, lib.st_token_workspace_bytes(args[1], rows, args[6], 2 * pairs))
-            _lib.check(lib.st_preference_loss_fwd(*args, *_label_args(labels, ignore), _ptr(cu), pairs, _ptr(ref), kind, average, beta, smoothing,
-                                                  scale, loss.data_ptr(), rewards.data_ptr(), row_grad if need else None, work,
-                                                  _lib.stream_ptr()), "st_preference_loss_fwd")
+        loss, rewards, buffer = _preference_fwd(x, call, True)
         ctx.mark_non_differentiable(rewards)
-        if need:
-            ctx.call, ctx.grad = (args, 1.0, ignore), None
-            ctx.save_for_backward(x, labels, buffer)
+        ctx.call, ctx.grad = (call[0], 1.0, call[2]), None
+        ctx.save_for_backward(x, call[1], buffer)
         return loss, rewards
 
     @staticmethod
@@ -286,8 +294,8 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: Optio
         labels, cu = labels.new_full((1,), ignore), labels.new_zeros(sequences + 1, dtype=torch.int32)
         logits = torch.cat([logits.reshape(0, logits.shape[-1]), logits.new_zeros(1, logits.shape[-1])])
         args = _logits_args(logits)
-    loss, rewards = _PreferenceFunction.apply(logits, (args, labels, ignore, cu, pairs, ref, _KINDS[kind], int(bool(average)), beta,
-                                                       label_smoothing, float(scale)))
+    call = (args, labels, ignore, cu, pairs, ref, _KINDS[kind], int(bool(average)), beta, label_smoothing, float(scale))
+    loss, rewards = _PreferenceFunction.apply(logits, call) if _wants_grad(logits) else _preference_fwd(logits, call, False)[:2]
     return PreferenceOutput(loss, rewards[:pairs], rewards[pairs:])
 
 
@@ -296,24 +304,28 @@ def _no_loss(logits: torch.Tensor) -> torch.Tensor:
     return logits.float().sum()
 
 
+def _policy_fwd(x, call, need):
+    args, labels, ignore, tau, cu, sequences, old, adv, ref, low, high, kl, ent, per_sequence, scale = call
+    lib = _lib.load()
+    rows = args[2]
+    loss, stats = _f32(x), _f32(x, 4)
+    grad = _grad_buffer(x) if need else None
+    with _on(x):
+        buffer, row_grad, work = _scratch(x, 16 * rows if need else 0, lib.st_token_workspace_bytes(args[1], rows, args[6], sequences))
+        _lib.check(lib.st_policy_loss_fwd(*args, *_label_args(labels, ignore), tau, _ptr(cu), sequences, old.data_ptr(), adv.data_ptr(),
+                                          int(adv.shape != labels.shape), _ptr(ref), low, high, kl, ent, per_sequence, scale,
+                                          loss.data_ptr(), stats.data_ptr(), row_grad if need else None, _ptr(grad), work,
+                                          _lib.stream_ptr()), "st_policy_loss_fwd")
+    return loss, stats, grad, buffer
+
+
 class _PolicyFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        args, labels, ignore, tau, cu, sequences, old, adv, ref, low, high, kl, ent, per_sequence, scale = call
-        lib = _lib.load()
-        rows, need = args[2], ctx.needs_input_grad[0]
-        loss, stats = _f32(x), _f32(x, 4)
-        grad = _grad_buffer(x) if need else None
-        with _on(x):
-            buffer, row_grad, work = _scratch(x, 16 * rows if need else 0, lib.st_token_workspace_bytes(args[1], rows, args[6], sequences))
-            _lib.check(lib.st_policy_loss_fwd(*args, *_label_args(labels, ignore), tau, _ptr(cu), sequences, old.data_ptr(), adv.data_ptr(),
-                                              int(adv.shape != labels.shape), _ptr(ref), low, high, kl, ent, per_sequence, scale,
-                                              loss.data_ptr(), stats.data_ptr(), row_grad if need else None, _ptr(grad), work,
-                                              _lib.stream_ptr()), "st_policy_loss_fwd")
+        loss, stats, ctx.grad, buffer = _policy_fwd(x, call, True)
         ctx.mark_non_differentiable(stats)
-        if need:
-            ctx.call, ctx.grad = (args, tau, ignore), grad
-            ctx.save_for_backward(x, labels, buffer)
+        ctx.call = call[0], call[3], call[2]
+        ctx.save_for_backward(x, call[1], buffer)
         return loss, stats
 
     @staticmethod
@@ -355,27 +367,32 @@ def clipped_policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: t
     tau, ignore = _temperature(temperature), _ignore(ignore_index)
     if labels.numel() == 0:
         return PolicyOutput(_no_loss(logits), torch.zeros(4, device=logits.device))
-    return PolicyOutput(*_PolicyFunction.apply(logits, (args, labels, ignore, tau, cu, sequences, old, adv, ref, clip_low, clip_high, kl_coef,
-                                                        entropy_coef, _REDUCTIONS[reduction], float(scale))))
+    call = (args, labels, ignore, tau, cu, sequences, old, adv, ref, clip_low, clip_high, kl_coef, entropy_coef, _REDUCTIONS[reduction],
+            float(scale))
+    return PolicyOutput(*(_PolicyFunction.apply(logits, call) if _wants_grad(logits) else _policy_fwd(logits, call, False)[:2]))
 
 
 # ---- distillation -------------------------------------------------------------------------------------------------------------
+def _distill_fwd(x, call, need):
+    args, idx, val, mask, tau, tail, scale = call
+    lib = _lib.load()
+    rows = args[2]
+    loss = _f32(x)
+    grad = _grad_buffer(x) if need else None
+    entries = (idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1])
+    with _on(x):
+        buffer, row_grad, work = _scratch(x, 32 * rows if need else 0, lib.st_distill_workspace_bytes(rows))
+        _lib.check(lib.st_distill_loss_fwd(*args, *entries, _ptr(mask), tau, tail, scale, loss.data_ptr(), row_grad if need else None,
+                                           _ptr(grad), work, _lib.stream_ptr()), "st_distill_loss_fwd")
+    return loss, grad, buffer
+
+
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        args, idx, val, mask, tau, tail, scale = call
-        lib = _lib.load()
-        rows, need = args[2], ctx.needs_input_grad[0]
-        loss = _f32(x)
-        grad = _grad_buffer(x) if need else None
-        entries = (idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1])
-        with _on(x):
-            buffer, row_grad, work = _scratch(x, 32 * rows if need else 0, lib.st_distill_workspace_bytes(rows))
-            _lib.check(lib.st_distill_loss_fwd(*args, *entries, _ptr(mask), tau, tail, scale, loss.data_ptr(), row_grad if need else None,
-                                               _ptr(grad), work, _lib.stream_ptr()), "st_distill_loss_fwd")
-        if need:
-            ctx.call, ctx.grad = (args, tau, tail), grad
-            ctx.save_for_backward(x, idx, val, buffer)
+        loss, ctx.grad, buffer = _distill_fwd(x, call, True)
+        ctx.call = call[0], call[4], call[5]
+        ctx.save_for_backward(x, call[1], call[2], buffer)
         return loss
 
     @staticmethod
@@ -421,7 +438,8 @@ def topk_distill_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     tau = _temperature(temperature)
     if idx.numel() == 0:
         return _no_loss(logits)
-    return _DistillFunction.apply(logits, (args, idx, val, mask, tau, int(bool(tail)), float(scale)))
+    call = (args, idx, val, mask, tau, int(bool(tail)), float(scale))
+    return _DistillFunction.apply(logits, call) if _wants_grad(logits) else _distill_fwd(logits, call, False)[0]
 
 
 # ---- modules ------------------------------------------------------------------------------------------------------------------

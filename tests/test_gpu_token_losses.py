@@ -641,6 +641,37 @@ def test_upstream_gradients_scale_and_repeat(vocab):
         assert torch.allclose(quarter, one / 4, rtol=8 * U, atol=tiny)
 
 
+def test_without_a_gradient_none_is_made():
+    """Under no_grad, or for logits that need none, the value alone: nothing of the logits' size is allocated."""
+    from style_transfer_amd import losses
+    x, t, idx, val = batch(8, 20000)
+    leaf = x.clone().requires_grad_(True)
+    old = losses.token_logprobs(x, t)
+    for fn in (lambda v: losses.token_logprobs(v, t), lambda v: losses.preference_loss(v, t).loss,
+               lambda v: losses.clipped_policy_loss(v, t, old, old + 5).loss, lambda v: losses.topk_distill_loss(v, idx, val, tail=True)):
+        for v, mode in ((leaf, torch.no_grad()), (leaf, torch.inference_mode()), (x, torch.enable_grad())):
+            with mode:
+                torch.cuda.synchronize()
+                torch.cuda.reset_peak_memory_stats()
+                before = torch.cuda.memory_allocated()
+                out = fn(v)
+                assert not out.requires_grad and torch.cuda.max_memory_allocated() - before < x.numel()
+        assert torch.equal(fn(leaf).detach(), out)
+
+
+def test_nothing_counts():
+    from style_transfer_amd import losses
+    x, t, idx, val = batch(8)
+    leaf = x.clone().requires_grad_(True)
+    got = losses.topk_distill_loss(leaf, idx, val, torch.zeros_like(t, dtype=torch.bool), tail=True)
+    got.backward()
+    assert float(got.detach()) == 0 and not leaf.grad.any()
+    leaf.grad = None
+    got = losses.preference_loss(leaf, torch.full_like(t, -100), beta=0.3)
+    got.loss.backward()
+    assert abs(float(got.loss.detach()) - math.log(2)) < 1e-6 and not leaf.grad.any()
+
+
 def test_a_changed_input_is_noticed():
     from style_transfer_amd import losses
     x, t, _, _ = batch(8)
