@@ -393,7 +393,7 @@ int launch_list_grad_t(const char* who, const Logits& p, const ListIn& q, const 
   const int chunk = bytes <= 4096 ? p.vocab : 16384 / (int)sizeof(T);
   const int splits = (int)st::cdivll(p.vocab, chunk);
   // a launch that may have nothing to do is kept small
-  const long long blocks = std::min<long long>(st::cdivll((long long)p.rows * splits, NT / tpr), skip ? 4096 : 0x7fffffffLL);
+  const long long blocks = std::min<long long>(st::cdivll((long long)p.rows * splits, NT / tpr), skip ? 4096 : 1LL << 23);
   if (tpr == 64) hipLaunchKernelGGL((list_grad_kernel<T, 64>), dim3((unsigned)blocks), dim3(NT), 0, s, p, q, gout, skip, splits, chunk, (T*)grad);
   else hipLaunchKernelGGL((list_grad_kernel<T, NT>), dim3((unsigned)blocks), dim3(NT), 0, s, p, q, gout, skip, splits, chunk, (T*)grad);
   return st::check_launch(who);
@@ -441,7 +441,9 @@ extern "C" int st_distill_loss_fwd(const void* x, int dtype, long long rows, lon
         const int rc = st::allow_dynamic_lds(distill_kernel<T, S>, (size_t)(MAX_VOCAB / 8 + 64), opt_in, who);
         if (rc != ST_OK) return rc;
       }
-      hipLaunchKernelGGL((distill_kernel<T, S>), dim3((unsigned)st::cdivll(rows, S::ROWS)), dim3(S::BLOCK), lds, s, p, q, u, words, (T*)grad);
+      const long long blocks = st::cdivll(rows, S::ROWS);
+      if (!fits_a_launch(blocks, S::BLOCK)) return st::fail(ST_ERR_BAD_ARG, "%s: rows=%lld vocab=%d: too many for a launch", who, rows, vocab);
+      hipLaunchKernelGGL((distill_kernel<T, S>), dim3((unsigned)blocks), dim3(S::BLOCK), lds, s, p, q, u, words, (T*)grad);
       return ST_OK;
     });
     if (launched != ST_OK) return launched;

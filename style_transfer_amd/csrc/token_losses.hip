@@ -430,7 +430,7 @@ template <typename T>
 int launch_stats_t(const char* who, const Logits& p, const StatsOut& o, hipStream_t s) {
   const Split k = split_of(p.rows, p.vocab, (int)sizeof(T));
   const long long parts = (long long)p.rows * k.splits, blocks = st::cdivll(parts, NT / k.tpr);
-  if (blocks > 0x7fffffffLL) return st::fail(ST_ERR_BAD_ARG, "%s: too many rows", who);
+  if (!fits_a_launch(blocks, NT)) return st::fail(ST_ERR_BAD_ARG, "%s: rows=%u vocab=%d: too many for a launch", who, p.rows, p.vocab);
   const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(NT), 0, s, p, k.splits, k.chunk, o); };
   const bool keep = o.again && read_twice_from_cache(p, (int)sizeof(T));
   if (k.tpr == 64) keep ? launch(stats_kernel<T, 64, true>) : launch(stats_kernel<T, 64, false>);
@@ -453,7 +453,7 @@ int launch_grad_t(const char* who, const Logits& p, const GradIn& g, void* grad,
   const int chunk = bytes <= 4096 ? p.vocab : 16384 / (int)sizeof(T);
   const int splits = (int)st::cdivll(p.vocab, chunk);
   // a launch that may have nothing to do is kept small: 131072 blocks that end at once take 28 us, 4096 take 3
-  const long long blocks = std::min<long long>(st::cdivll((long long)p.rows * splits, NT / tpr), g.skip_if_one ? 4096 : 0x7fffffffLL);
+  const long long blocks = std::min<long long>(st::cdivll((long long)p.rows * splits, NT / tpr), g.skip_if_one ? 4096 : 1LL << 23);
   if (tpr == 64) hipLaunchKernelGGL((grad_kernel<T, 64>), dim3((unsigned)blocks), dim3(NT), 0, s, p, g, splits, chunk, (T*)grad);
   else hipLaunchKernelGGL((grad_kernel<T, NT>), dim3((unsigned)blocks), dim3(NT), 0, s, p, g, splits, chunk, (T*)grad);
   return st::check_launch(who);
@@ -589,13 +589,17 @@ extern "C" int st_policy_loss_fwd(const void* x, int dtype, long long rows, long
   // a block of 1024 threads: 16 sequences at a time, or four labels a thread
   u.blocks = (int)std::min<long long>(COUNT_BLOCKS, per_sequence ? st::cdivll(sequences, 16) : st::cdivll(rows, 4096));
   hipLaunchKernelGGL(count_kernel, dim3(u.blocks), dim3(1024), 0, s, p, q, u);
-  with_type(dtype, [&](auto type) {
+  rc = with_type(dtype, [&](auto type) {
     using T = decltype(type);
-    with_shape((long long)vocab * (long long)sizeof(T), [&](auto shape) {
+    return with_shape((long long)vocab * (long long)sizeof(T), [&](auto shape) -> int {
       using S = decltype(shape);
-      hipLaunchKernelGGL((policy_kernel<T, S>), dim3((unsigned)st::cdivll(rows, S::ROWS)), dim3(S::BLOCK), 0, s, p, q, u, (T*)grad);
+      const long long blocks = st::cdivll(rows, S::ROWS);
+      if (!fits_a_launch(blocks, S::BLOCK)) return st::fail(ST_ERR_BAD_ARG, "%s: rows=%lld vocab=%d: too many for a launch", who, rows, vocab);
+      hipLaunchKernelGGL((policy_kernel<T, S>), dim3((unsigned)blocks), dim3(S::BLOCK), 0, s, p, q, u, (T*)grad);
+      return ST_OK;
     });
   });
+  if (rc != ST_OK) return rc;
   launch_sum_terms(u, s);
   return st::check_launch(who);
 }

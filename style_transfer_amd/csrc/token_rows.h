@@ -683,6 +683,9 @@ struct Space {
 };
 
 
+// HIP counts the threads of a launch in 32 bits.
+inline bool fits_a_launch(long long blocks, int threads) { return blocks * threads <= 0xffffffffLL; }
+
 inline Sums make_sums(Space& w, long long rows, float* loss, float* stats, double scale, double kl, double ent) {
   Sums q{};
   q.counted = w.take<double>(COUNT_BLOCKS);
