@@ -502,8 +502,20 @@ struct Row : Span<T, TPR> {
       for (int j = 0; j < VEC; ++j) g = fmaxf(g, f[j]);
     }
     g = lanes_max(g);                                           // one reference for the wave, in a scalar register
+    if (g == -INFINITY) {                                       // nothing there (a mask): all that the wave holds
+#pragma unroll
+      for (int i = 1; i < NCH; ++i)
+        if (i < slots) {
+          float f[VEC];
+          elements(i, f);
+          leave_out.vector(i, t, f);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) g = fmaxf(g, f[j]);
+        }
+      g = lanes_max(g);
+    }
     const Ref ref = make_ref(g, c);
-    Part p{ref.m, 0.f, 0.f};
+    Part p{g, 0.f, 0.f};                                        // -inf still: an empty part, which no other one is seen from
     if (!ref.low) {
       add_up<1, false, WANT_W>(&beside, ref, c, p.s, p.w);
 #pragma unroll

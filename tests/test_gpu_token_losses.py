@@ -520,6 +520,42 @@ def test_distill_rows_of_every_size(dtype, vocab, tail):
     close(leaf.grad, want, distill_bound(x, idx, val, mask, tau, want, dtype), "gradient")
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1023), (torch.bfloat16, 8200), (torch.float32, 16387), (torch.float16, 60000),
+                                         (torch.float32, 65537), (torch.bfloat16, 170001)])
+def test_low_logits_behind_masked_ones(dtype, vocab):
+    """Logits far below 0 behind a masked beginning: the first vectors of some waves, or of all, hold nothing to start from."""
+    from style_transfer_amd.losses import clipped_policy_loss, topk_distill_loss, token_logprobs
+    x = logits(5, vocab, dtype, vocab) - 300.0
+    x[0, : vocab // 2] = -math.inf
+    x[1, : min(1000, vocab // 2)] = -math.inf
+    x[2, vocab // 3:] = -math.inf
+    x[3, : vocab - 3] = -math.inf                               # the last elements alone
+    x[4, ::2] = -math.inf
+    t = torch.tensor([vocab - 1, vocab - 2, 5, vocab - 2, 7])
+    logp, h, log_q, q = O.token_logprobs(x, t)
+    err = row_error(vocab) + logp.abs() * 2 * U
+    leaf = x.cuda().requires_grad_(True)
+    got, entropy = token_logprobs(leaf, t.cuda(), return_entropy=True)
+    close(got, logp, err, "logp")
+    close(entropy, h, (h + 2) * row_error(vocab) + 2 * h * U, "entropy")
+    seqs, adv = [(0, 5)], torch.tensor([1.0, -1.0, 2.0, 0.5, -0.5])
+    loss, stats, want = O.policy(x, t, seqs, logp.float(), adv, ent=0.1)
+    policy = clipped_policy_loss(leaf[None], t[None].cuda(), logp.float()[None].cuda(), adv[None].cuda(), entropy_coef=0.1)
+    policy.loss.backward()
+    close(policy.stats, stats, 14 * float(err.max()) + stats.abs() * 2 * U, "stats")
+    a, b = adv.abs().double() / 5, torch.full((5,), 0.02, dtype=torch.float64)
+    close(leaf.grad, want, grad_bound(want, dtype, log_q, a, b, h, extra=2 * float(err.max())), "policy gradient")
+    for tail in (False, True):
+        idx = torch.tensor([[vocab - 1, vocab - 2], [vocab - 2, vocab - 1], [5, 3], [vocab - 2, vocab - 1], [7, 9]])
+        val = torch.tensor([[-0.5, -1.5]]).repeat(5, 1)
+        loss, want = O.distill(x, idx, val, None, 1.0, tail)
+        leaf.grad = None
+        got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)
+        got.backward()
+        close(got, torch.tensor(loss), 2 * row_error(vocab) + 60 * U + abs(loss) * 8 * U, "loss")
+        close(leaf.grad, want, distill_bound(x, idx, val, None, 1.0, want, dtype), "distillation gradient")
+
+
 def test_a_padded_batch_in_place():
     """Rows of a slice at every alignment through the kernels that hold a row: as of a copy, and no other memory is written."""
     from style_transfer_amd import losses
