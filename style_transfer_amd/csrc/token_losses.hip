@@ -87,7 +87,7 @@ __global__ __launch_bounds__(NT) void stats_kernel(Logits p, int splits, int chu
   const unsigned r = (unsigned)(part / splits);
   const int sp = (int)(part % splits);
   const bool live = r < p.rows;
-  const long long label = live && p.labels ? load_index(p.labels, p.labels64, r) : p.ignore;
+  const long long label = live ? load_index(p.labels, p.labels64, r) : p.ignore;
   if (live && label != p.ignore) {
     const int lo = std::min((long long)sp * chunk, (long long)p.vocab), hi = std::min((long long)lo + chunk, (long long)p.vocab);
     const T* x = reinterpret_cast<const T*>(p.x) + row_offset(p, r) + lo;
@@ -303,16 +303,18 @@ __device__ __forceinline__ TokenTerms token_terms(double log_ratio, double d, co
   return t;
 }
 
-// The sequence of row r, or -1 outside of all: how many sequences end at or before r, 64 at a time.  A whole wave calls it.
+// The sequence of row r, or -1 outside of all: how many sequences end at or before r, found by 64 probes at a time (8192
+// sequences: three steps; one after another they were 128, and 32768 rows of 4096 bf16 took 168 us instead of 92).  A whole
+// wave calls it.
 __device__ __forceinline__ int sequence_of(const Sequences& q, unsigned r) {
   if (!q.cu) return (int)(r / q.inner);
-  unsigned s = 0;
-  for (unsigned first = 0; first < q.count; first += 64) {
-    const unsigned i = first + (threadIdx.x & 63);
-    s += (unsigned)__popcll(__ballot(i < q.count && q.cu[i + 1] <= (int)r));
-    if (s < first + 64) break;
+  unsigned lo = 0, hi = q.count;                                // the answer lies in [lo, hi]
+  while (lo < hi) {
+    const unsigned step = (hi - lo + 63) / 64, i = lo + ((threadIdx.x & 63) + 1) * step - 1;
+    lo += step * (unsigned)__popcll(__ballot(i < hi && q.cu[i + 1] <= (int)r));
+    hi = std::min(hi, lo + step - 1);
   }
-  return s < q.count && q.cu[s] <= (int)r ? (int)s : -1;
+  return lo < q.count && q.cu[lo] <= (int)r ? (int)lo : -1;
 }
 
 // What the mean divides by: labels of all rows, or of each sequence and how many sequences have any.
@@ -320,15 +322,17 @@ __global__ __launch_bounds__(1024) void count_kernel(Logits p, PolicyIn q, Sums 
   __shared__ double red[16];
   double n = 0;
   if (q.per_sequence) {
-    for (unsigned s = blockIdx.x * 16 + (threadIdx.x >> 6); s < q.seq.count; s += gridDim.x * 16) {
+    // a wave a sequence; of up to 64 sequences, which may be long, a block each (one of 32768 rows: the loss 230 us -> 108)
+    const bool alone = q.seq.count <= COUNT_BLOCKS;
+    const unsigned threads = alone ? 1024 : 64, t = threadIdx.x % threads, each = 1024 / threads;
+    for (unsigned s = blockIdx.x * each + threadIdx.x / threads; s < q.seq.count; s += gridDim.x * each) {
       unsigned start, end;
       sequence(q.seq, s, start, end);
-      int c = 0;
-      for (unsigned r = start + (threadIdx.x & 63); r < end; r += 64) c += load_index(p.labels, p.labels64, r) != p.ignore;
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) c += __shfl_xor(c, off, 64);
-      if ((threadIdx.x & 63) == 0) {
-        q.count[s] = c;
+      double c = 0;
+      for (unsigned r = start + t; r < end; r += threads) c += load_index(p.labels, p.labels64, r) != p.ignore;
+      c = alone ? block_sum64(c, red) : lanes_sum(c);           // alone: the same s for the whole block
+      if (t == 0) {
+        q.count[s] = (int)c;
         n += c > 0;
       }
     }
@@ -341,9 +345,7 @@ __global__ __launch_bounds__(1024) void count_kernel(Logits p, PolicyIn q, Sums 
     for (unsigned r = first + blockIdx.x * 1024 + threadIdx.x; r < end; r += gridDim.x * 1024) n += load_index(p.labels, p.labels64, r) != p.ignore;
   }
   n = block_sum64(n, red);
-  if (threadIdx.x == 0) {
-    u.counted[blockIdx.x] = n;
-  }
+  if (threadIdx.x == 0) u.counted[blockIdx.x] = n;
 }
 
 // One pass: a row's statistics, its terms and, where the caller wants one, its gradient (for an upstream gradient of 1).
@@ -586,8 +588,9 @@ extern "C" int st_policy_loss_fwd(const void* x, int dtype, long long rows, long
   q.scale = scale;
   q.per_sequence = per_sequence;
   q.row = reinterpret_cast<RowGrad*>(row_grad);
-  // a block of 1024 threads: 16 sequences at a time, or four labels a thread
-  u.blocks = (int)std::min<long long>(COUNT_BLOCKS, per_sequence ? st::cdivll(sequences, 16) : st::cdivll(rows, 4096));
+  // a block of 1024 threads: a sequence or 16 at a time, or four labels a thread
+  u.blocks = (int)std::min<long long>(COUNT_BLOCKS, !per_sequence ? st::cdivll(rows, 4096) : sequences <= COUNT_BLOCKS ? sequences
+                                                                                                               : st::cdivll(sequences, 16));
   hipLaunchKernelGGL(count_kernel, dim3(u.blocks), dim3(1024), 0, s, p, q, u);
   rc = with_type(dtype, [&](auto type) {
     using T = decltype(type);

@@ -354,6 +354,38 @@ def test_rows_outside_the_sequences_do_not_count():
         assert not leaf.grad[[0, 1, 7]].any()
 
 
+@pytest.mark.parametrize("rows,sequences", [(700, 1), (900, 64), (900, 65), (3000, 700), (20000, 5000), (300000, 70000)])
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_policy_over_many_rows_and_sequences(rows, sequences, reduction):
+    """One sequence to tens of thousands, empty ones among them, more rows than one block adds up; the formula in 64 bits."""
+    from style_transfer_amd.losses import clipped_policy_loss
+    vocab = 3
+    g = torch.Generator().manual_seed(rows + sequences)
+    x, t = logits(rows, vocab, torch.float32, rows, 1.0), torch.randint(0, vocab, (rows,), generator=g)
+    t[torch.rand(rows, generator=g) < 0.3] = -100
+    cu = torch.cat([torch.tensor([2, rows - 3]), torch.randint(2, rows - 2, (sequences - 1,), generator=g)]).sort().values
+    adv, old = rand(1, sequences), torch.full((rows,), -1.0)
+    lengths = cu[1:] - cu[:-1]
+    of = torch.full((rows,), -1)
+    of[2:rows - 3] = torch.repeat_interleave(torch.arange(sequences), lengths)
+    keep = (t != -100) & (of >= 0)
+    count = torch.zeros(sequences, dtype=torch.float64).index_add_(0, of[keep], torch.ones(int(keep.sum()), dtype=torch.float64))
+    w = torch.where(keep, 1 / count[of] / (count > 0).sum() if reduction == "sequence" else 1 / count.sum(), 0.0)
+    z = x.double().requires_grad_(True)
+    logp = torch.log_softmax(z, 1).gather(1, t.clamp(min=0)[:, None])[:, 0]
+    ratio, a = (logp - old.double()).exp(), adv.double()[of]
+    each = -torch.minimum(ratio * a, ratio.clamp(0.8, 1.2) * a)
+    want = (w * each).sum()
+    want.backward()
+    leaf = x.cuda().requires_grad_(True)
+    got = clipped_policy_loss(leaf, t.cuda(), old.cuda(), adv.cuda(), cu_seqlens=cu.int().cuda(), reduction=reduction)
+    got.loss.backward()
+    # a row: its logarithm's and its exponential's error, relative to a ratio of at most e; entries: as much of the row's weight
+    row = row_error(vocab) * math.e * a.abs()
+    close(got.loss, want.detach(), float((w * row).sum()) + 4 * U * float(w @ each.detach().abs()), "loss")
+    close(leaf.grad, z.grad, (w * row)[:, None] * 2 + 4 * U * z.grad.abs() + 2.0 ** -126, "gradient")
+
+
 # ---- distillation -------------------------------------------------------------------------------------------------------------
 def teacher(x, k, tau, tail, seed):
     g = torch.Generator().manual_seed(seed)
