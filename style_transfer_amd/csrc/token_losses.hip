@@ -200,7 +200,7 @@ __global__ __launch_bounds__(1024) void pref_kernel(Logits p, PrefIn q) {
   for (int side = 0; side < 2; ++side) {
     sequence(q.seq, pair + side * pairs, start[side], end[side]);
     sum[side] = n[side] = 0;
-    for (unsigned r = start[side] + threadIdx.x; r < end[side]; r += 1024) {
+    for (unsigned r = start[side] + threadIdx.x; r < end[side]; r += blockDim.x) {
       sum[side] += (double)q.logp[r];
       n[side] += load_index(p.labels, p.labels64, r) != p.ignore;
     }
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(1024) void pref_kernel(Logits p, PrefIn q) {
   if (q.row)
     for (int side = 0; side < 2; ++side) {
       const float a = (float)slopes[side], patch = (float)(slopes[side] * p.inv_tau);
-      for (unsigned r = start[side] + threadIdx.x; r < end[side]; r += 1024) {
+      for (unsigned r = start[side] + threadIdx.x; r < end[side]; r += blockDim.x) {
         const f32x4 s = q.state[r];
         const bool counts = load_index(p.labels, p.labels64, r) != p.ignore && s[1] != 0.f;
         q.row[r] = counts ? f32x4{s[0], -a * s[1], 0.f, patch} : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -553,7 +553,8 @@ extern "C" int st_preference_loss_fwd(const void* x, int dtype, long long rows, 
   q.rewards = rewards;
   q.row = o.clear;
   if ((rc = launch_stats(who, dtype, p, o, s)) != ST_OK) return rc;
-  hipLaunchKernelGGL(pref_kernel, dim3((unsigned)pairs), dim3(1024), 0, s, p, q);
+  // 4096 pairs of 8 tokens: 90 us with 256 threads a pair, 126 with 1024 (32768 rows of 4096 bf16)
+  hipLaunchKernelGGL(pref_kernel, dim3((unsigned)pairs), dim3(rows <= 512LL * pairs ? 256 : 1024), 0, s, p, q);
   hipLaunchKernelGGL(pref_mean_kernel, dim3(1), dim3(256), 0, s, q);
   return st::check_launch(who);
 }
