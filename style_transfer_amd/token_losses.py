@@ -178,7 +178,7 @@ class _TokenLogProbsFunction(torch.autograd.Function):
     def forward(ctx, x, call):
         args, labels, tau, ignore, want_entropy = call
         logp, entropy, buffer = _logprobs_fwd(x, args, labels, tau, ignore, want_entropy, True)
-        ctx.call = args, tau, ignore
+        ctx.call = tau, ignore
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, labels, buffer)
         return (logp, entropy) if want_entropy else logp
@@ -189,12 +189,12 @@ class _TokenLogProbsFunction(torch.autograd.Function):
         if g_logp is None and g_entropy is None:
             return None, None
         x, labels, state = ctx.saved_tensors
-        args, tau, ignore = ctx.call
+        tau, ignore = ctx.call
         grad = _grad_buffer(x)
         g_logp = None if g_logp is None else _gout(g_logp)
         g_entropy = None if g_entropy is None else _gout(g_entropy)
         with _on(x):
-            _lib.check(_lib.load().st_token_logprobs_bwd(*args, *_label_args(labels, ignore), tau, state.data_ptr(), _ptr(g_logp), _ptr(g_entropy),
+            _lib.check(_lib.load().st_token_logprobs_bwd(*_logits_args(x), *_label_args(labels, ignore), tau, state.data_ptr(), _ptr(g_logp), _ptr(g_entropy),
                                                          grad.data_ptr(), _lib.stream_ptr()), "st_token_logprobs_bwd")
         return grad, None
 
@@ -225,12 +225,12 @@ def _take_grad(ctx, x):
 
 
 def _token_loss_bwd(ctx, gout):
-    x, labels, row_grad = ctx.saved_tensors
-    args, tau, ignore = ctx.call
+    x, labels, row_grad = ctx.saved_tensors                    # x may be a copy elsewhere (saved-tensor hooks): its own address
+    tau, ignore = ctx.call
     grad, for_one = _take_grad(ctx, x)
     gout = _gout(gout)
     with _on(x):
-        _lib.check(_lib.load().st_token_loss_bwd(*args, *_label_args(labels, ignore), tau, row_grad.data_ptr(), gout.data_ptr(), for_one,
+        _lib.check(_lib.load().st_token_loss_bwd(*_logits_args(x), *_label_args(labels, ignore), tau, row_grad.data_ptr(), gout.data_ptr(), for_one,
                                                  grad.data_ptr(), _lib.stream_ptr()), "st_token_loss_bwd")
     return grad, None
 
@@ -253,7 +253,7 @@ class _PreferenceFunction(torch.autograd.Function):
     def forward(ctx, x, call):
         loss, rewards, buffer = _preference_fwd(x, call, True)
         ctx.mark_non_differentiable(rewards)
-        ctx.call, ctx.grad = (call[0], 1.0, call[2]), None
+        ctx.call, ctx.grad = (1.0, call[2]), None
         ctx.save_for_backward(x, call[1], buffer)
         return loss, rewards
 
@@ -324,7 +324,7 @@ class _PolicyFunction(torch.autograd.Function):
     def forward(ctx, x, call):
         loss, stats, ctx.grad, buffer = _policy_fwd(x, call, True)
         ctx.mark_non_differentiable(stats)
-        ctx.call = call[0], call[3], call[2]
+        ctx.call = call[3], call[2]
         ctx.save_for_backward(x, call[1], buffer)
         return loss, stats
 
@@ -391,7 +391,7 @@ class _DistillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
         loss, ctx.grad, buffer = _distill_fwd(x, call, True)
-        ctx.call = call[0], call[4], call[5]
+        ctx.call = call[4], call[5]
         ctx.save_for_backward(x, call[1], call[2], buffer)
         return loss
 
@@ -399,11 +399,11 @@ class _DistillFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         x, idx, val, row_grad = ctx.saved_tensors
-        args, tau, tail = ctx.call
+        tau, tail = ctx.call
         grad, for_one = _take_grad(ctx, x)
         gout = _gout(gout)
         with _on(x):
-            _lib.check(_lib.load().st_distill_loss_bwd(*args, idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1], tau, tail,
+            _lib.check(_lib.load().st_distill_loss_bwd(*_logits_args(x), idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1], tau, tail,
                                                        row_grad.data_ptr(), gout.data_ptr(), for_one, grad.data_ptr(), _lib.stream_ptr()),
                        "st_distill_loss_bwd")
         return grad, None

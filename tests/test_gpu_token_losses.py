@@ -740,6 +740,29 @@ def test_nothing_counts():
     assert abs(float(got.loss.detach()) - math.log(2)) < 1e-6 and not leaf.grad.any()
 
 
+@pytest.mark.parametrize("vocab", [700, 20000])
+def test_logits_kept_elsewhere_until_the_backward(vocab):
+    """Saved tensors moved to the host and back: the backward reads the copy, whose address and strides are its own."""
+    from style_transfer_amd import losses
+    x, t, idx, val = batch(6, vocab)
+    old = losses.token_logprobs(x, t) + 0.1
+    wide = torch.cat([x, x], 2)
+    for weight in (1.0, 3.0):
+        for fn in (lambda v: losses.token_logprobs(v, t).sum(), lambda v: losses.preference_loss(v, t).loss,
+                   lambda v: losses.clipped_policy_loss(v, t, old, old + 9).loss, lambda v: losses.topk_distill_loss(v, idx, val, tail=True)):
+            grads = []
+            for away in (False, True):
+                leaf = wide.clone().requires_grad_(True)
+                with torch.autograd.graph.save_on_cpu() if away else torch.enable_grad():
+                    loss = weight * fn((leaf * 1)[:, :, 3:vocab + 3])
+                other = torch.full_like(wide, math.nan)        # takes the place of what was let go
+                loss.backward()
+                grads.append(leaf.grad)
+                del other
+            half = 2 * row_error(vocab)
+            assert torch.allclose(grads[0], grads[1], rtol=half, atol=half * float(grads[0].abs().max()))
+
+
 def test_a_changed_input_is_noticed():
     from style_transfer_amd import losses
     x, t, _, _ = batch(8)
