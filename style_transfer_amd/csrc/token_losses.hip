@@ -137,7 +137,7 @@ __device__ __forceinline__ RowGrad row_grad(const Logits& p, const GradIn& g, un
   if (!counts) return v;
   if (g.row) {
     v = g.row[r];
-    v[1] *= scale; v[2] *= scale; v[3] *= scale;
+    for (int i = 1; i < 4; ++i) v[i] = v[i] == 0.f ? 0.f : v[i] * scale;      // a row without a gradient has none, whatever comes from above
     return v;
   }
   const f32x4 s = g.state[r];
