@@ -18,6 +18,7 @@ namespace {
 using namespace st_token;
 
 constexpr int MAX_VOCAB = 1 << 20;       // the bitmap of a row: 128 KB of LDS
+constexpr int MAX_LIST = 4096;           // a list that names a token twice is gone through once for each entry
 constexpr size_t MAX_PLAIN_LDS = 48 << 10;   // dynamic LDS that a kernel gets without asking (64 KB with what it declares)
 
 // what the list of a row, or a wave's part of it, says by itself
@@ -212,13 +213,10 @@ __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn
   for (int k = threadIdx.x & 63; k < q.k; k += 64) {
     const int j = entry_index(q, first + k, p.vocab);
     bool again = false;
-    for (int i = 0; j >= 0 && i < k && !again; ++i) again = entry_index(q, first + i, p.vocab) == j;
-    if (again) {
-      n += 1;
-    } else if (j >= 0) {
-      const float d = distance((float)x[j], ref, p.c), e = __builtin_amdgcn_exp2f(d);
-      s += e;
-    }
+    if (j >= 0)
+      for (int i = 0; i < k; ++i) again |= entry_index(q, first + i, p.vocab) == j;      // no exit: the loads overlap
+    if (again) n += 1;
+    else if (j >= 0) s += __builtin_amdgcn_exp2f(distance((float)x[j], ref, p.c));
   }
   o.s = lanes_sum(s);
   o.used -= (int)lanes_sum(n);
@@ -414,7 +412,7 @@ extern "C" int st_distill_loss_fwd(const void* x, int dtype, long long rows, lon
   int rc;
   if (bad_logits(who, p, dtype, rows, inner, s_outer, s_inner, &rc)) return rc;
   ST_REQUIRE(rows > 0 && k > 0, "%s: rows=%lld k=%d", who, rows, k);
-  ST_REQUIRE(vocab <= MAX_VOCAB, "%s: vocab=%d (at most %d)", who, vocab, MAX_VOCAB);
+  ST_REQUIRE(vocab <= MAX_VOCAB && k <= MAX_LIST, "%s: vocab=%d (at most %d), k=%d (at most %d)", who, vocab, MAX_VOCAB, k, MAX_LIST);
   ST_REQUIRE(teacher_idx && teacher_val && loss && workspace, "%s: null pointer", who);
   hipStream_t s = (hipStream_t)stream;
   Space w{reinterpret_cast<char*>(workspace)};
@@ -460,7 +458,8 @@ extern "C" int st_distill_loss_bwd(const void* x, int dtype, long long rows, lon
   int rc;
   if (bad_logits(who, p, dtype, rows, inner, s_outer, s_inner, &rc)) return rc;
   if (rows == 0) return ST_OK;
-  ST_REQUIRE(teacher_idx && teacher_val && row_grad && grad && k > 0, "%s: null pointer", who);
+  ST_REQUIRE(vocab <= MAX_VOCAB && k > 0 && k <= MAX_LIST, "%s: vocab=%d (at most %d), k=%d (at most %d)", who, vocab, MAX_VOCAB, k, MAX_LIST);
+  ST_REQUIRE(teacher_idx && teacher_val && row_grad && grad, "%s: null pointer", who);
   ListIn q{};
   q.idx = teacher_idx;
   q.idx64 = idx64;

@@ -421,7 +421,7 @@ def topk_distill_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     they are the teacher's log-probabilities (at ``temperature``, over its whole vocabulary), and all tokens that are not listed
     form one more entry of the sum, with ``1 - sum_k p_k`` and the student's probability of the same tokens.
 
-    At most 2^20 tokens.  A position with no used entry contributes 0.  An index of ``V`` or more makes its position's loss and
+    At most 2^20 tokens and 4096 entries.  A position with no used entry contributes 0.  An index of ``V`` or more makes its position's loss and
     gradient NaN."""
     args = _logits_args(logits)
     shape = logits.shape[:-1]

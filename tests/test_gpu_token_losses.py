@@ -473,6 +473,29 @@ def test_distill_repeated_unused_and_foreign_entries(tail, vocab):
     assert float(got.detach()) == 0 and none.grad.shape == (0, vocab)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("vocab,k", [(5000, 4096), (300, 500), (60000, 1500)])
+def test_distill_long_lists(tail, vocab, k):
+    """More entries than a row has threads, or tokens: drawn with repeats."""
+    from style_transfer_amd.losses import topk_distill_loss
+    x = logits(3, vocab, torch.float32, k)
+    idx = torch.randint(0, vocab, (3, k), generator=torch.Generator().manual_seed(vocab))
+    idx[1] = torch.where(torch.rand(k, generator=torch.Generator().manual_seed(1)) < 0.5, -1, idx[1])
+    val = torch.log_softmax(rand(k, 3, k), 1) - 0.2 if tail else rand(k, 3, k)
+    loss, want = O.distill(x, idx, val, None, 1.0, tail)
+    leaf = x.cuda().requires_grad_(True)
+    got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)
+    got.backward()
+    # the list's own sums: K / 64 entries a lane where a wave goes through them, as for a row
+    more = k / 64 * U
+    close(got, torch.tensor(loss), 2 * row_error(vocab) + 60 * U + 4 * more + abs(loss) * 4 * U, "loss")
+    q = torch.stack([O.row(r, 1.0)[1] for r in x])
+    listed = torch.zeros(3, vocab, dtype=torch.float64)         # what the list subtracts, a token's entries added up
+    p = (val.double() if tail else torch.log_softmax(val.double().masked_fill(idx < 0, -math.inf), 1)).exp() * (idx >= 0)
+    listed.scatter_add_(1, idx.clamp(min=0), p)
+    close(leaf.grad, want, distill_bound(x, idx, val, None, 1.0, want, torch.float32) + (q + listed) / 3 * (4 * more + 40 * U), "gradient")
+
+
 def test_distill_keeps_what_little_the_rest_holds():
     """The student is sure of a listed token: 1 - sum q has no digit left, the sum off the list has all of them."""
     from style_transfer_amd.losses import topk_distill_loss
@@ -725,6 +748,45 @@ def test_without_a_gradient_none_is_made():
                 out = fn(v)
                 assert not out.requires_grad and torch.cuda.max_memory_allocated() - before < x.numel()
         assert torch.equal(fn(leaf).detach(), out)
+
+
+@pytest.mark.parametrize("vocab", [700, 20000])
+def test_an_upstream_gradient_that_is_no_number(vocab):
+    """It reaches the rows that count and no other: those stay 0."""
+    from style_transfer_amd import losses
+    x, t, idx, val = batch(5, vocab)
+    flat, cu = x.view(24, -1), torch.tensor([0, 6, 12, 15, 20], dtype=torch.int32, device="cuda")
+    labels = torch.where(t.view(-1) == -100, 0, t.view(-1))
+    old = losses.token_logprobs(flat, labels) + 0.1
+    mask = torch.arange(24, device="cuda") < 20
+    for fn in (lambda v: losses.preference_loss(v, labels, cu_seqlens=cu).loss,
+               lambda v: losses.clipped_policy_loss(v, labels, old, old + 20, cu_seqlens=cu).loss,
+               lambda v: losses.topk_distill_loss(v, idx.view(24, -1), val.view(24, -1), mask, tail=True)):
+        for up in (math.nan, math.inf):
+            leaf = flat.clone().requires_grad_(True)
+            (fn(leaf) * up).backward()
+            assert not leaf.grad[20:].any() and not torch.isfinite(leaf.grad[:20]).all(1).any()
+
+
+def test_gradients_beyond_32_bits():
+    """Broadcast logits whose gradient rows reach past 2^32 elements: every row as the first of its kind."""
+    from style_transfer_amd import losses
+    vocab, rows = 40001, 107500
+    assert rows * vocab > 2 ** 32
+    x = (logits(1, vocab, torch.bfloat16, 3)).cuda()
+    t = torch.arange(rows, device="cuda") % 5
+    old = torch.full((rows,), -9.0, device="cuda")
+    idx, val = (torch.arange(4, device="cuda") * 7).expand(rows, 4).contiguous(), torch.full((rows, 4), -2.0, device="cuda")
+    for fn in (lambda v: losses.clipped_policy_loss(v[None], t[None], old[None], old[None] + 10).loss,
+               lambda v: losses.topk_distill_loss(v, idx, val, tail=True), lambda v: losses.token_logprobs(v, t).sum()):
+        view = x.expand(rows, vocab).detach().requires_grad_(True)
+        grad, = torch.autograd.grad(fn(view), [view])
+        few = grad[:5].clone()
+        assert few.any()
+        for first in range(0, rows, 21500):                     # whole groups of five
+            part = grad[first:first + 21500].view(-1, 5, vocab)
+            assert torch.equal(part, few[None].expand_as(part))
+        del grad, part, view
 
 
 def test_nothing_counts():

@@ -100,6 +100,7 @@ def test_c_entries_return_errors():
     assert policy(2, 0.2) == -1 and policy(1, 1.5) == -1
     assert lib.st_distill_loss_fwd(*good, p, 1, p, 0, None, 1.0, 0, 1.0, p, None, None, p, None) == -1
     assert lib.st_distill_loss_fwd(p, 0, 4, 4, 0, 2 ** 21, 2 ** 21, p, 1, p, 3, None, 1.0, 0, 1.0, p, None, None, p, None) == -1
+    assert lib.st_distill_loss_fwd(*good, p, 1, p, 4097, None, 1.0, 0, 1.0, p, None, None, p, None) == -1 and b"4096" in lib.st_last_error()
     many = (p, 0, 2 ** 31 - 1, 2 ** 31 - 1, 0, 10, 10)         # more threads than a launch has
     assert lib.st_token_logprobs_fwd(*many, *labels, 1.0, p, None, None, p, None) == -1 and b"launch" in lib.st_last_error()
     assert lib.st_token_workspace_bytes(0, -1, 10, 0) == 0 and lib.st_token_workspace_bytes(1, 1, 131072, 2) > 0
