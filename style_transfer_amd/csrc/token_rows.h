@@ -694,7 +694,6 @@ struct Space {
   }
 };
 
-
 // HIP counts the threads of a launch in 32 bits.
 inline bool fits_a_launch(long long blocks, int threads) { return blocks * threads <= 0xffffffffLL; }
 
