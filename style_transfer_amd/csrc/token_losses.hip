@@ -18,24 +18,36 @@ __device__ __forceinline__ float load_one(const void* base, long long i) {
   return (float)reinterpret_cast<const T*>(base)[i];
 }
 
+struct StatsOut {
+  float* logp;           // or
+  double* wide;          // for sums over sequences, of which a loss takes differences
+  float* entropy;
+  f32x4* state;
+  f32x4* parts;          // [rows][splits], used where splits > 1
+  RowGrad* clear;        // row gradients that a loss kernel fills in for the rows it owns
+  int again;             // a gradient pass will read the logits again
+};
+
 // A row's outputs from its joined statistics: log-probability, entropy, and what the gradient needs.  `state`:
 // (m, 1 / (tau S), H - ln S, -).
 template <typename T>
-__device__ __forceinline__ void write_row(const Logits& p, unsigned r, long long label, const Part& q, float* logp, float* entropy,
-                                          f32x4* state) {
+__device__ __forceinline__ void write_row(const Logits& p, unsigned r, long long label, const Part& q, const StatsOut& o) {
   const RowStat st = finish<true>(q, p);
-  float lp = NAN, h = st.h, inv = st.inv_ts;
-  if (label >= 0 && label < p.vocab) lp = (float)log_prob(load_one<T>(p.x, row_offset(p, r) + label), st, p);
+  double lp = NAN;
+  float inv = st.inv_ts;
+  if (label >= 0 && label < p.vocab) lp = log_prob(load_one<T>(p.x, row_offset(p, r) + label), st, p);
   else inv = NAN;                                              // a label outside the vocabulary: visible, never an access
-  logp[r] = lp;
-  if (entropy) entropy[r] = h;
-  if (state) state[r] = f32x4{st.ref, inv, st.inv_ts == 0.f ? 0.f : (float)((double)st.h - st.ln_s), 0.f};
+  if (o.logp) o.logp[r] = (float)lp;
+  if (o.wide) o.wide[r] = lp;
+  if (o.entropy) o.entropy[r] = st.h;
+  if (o.state) o.state[r] = f32x4{st.ref, inv, st.inv_ts == 0.f ? 0.f : (float)((double)st.h - st.ln_s), 0.f};
 }
 
-__device__ __forceinline__ void write_no_row(unsigned r, float* logp, float* entropy, f32x4* state) {
-  logp[r] = 0.f;
-  if (entropy) entropy[r] = 0.f;
-  if (state) state[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ void write_no_row(unsigned r, const StatsOut& o) {
+  if (o.logp) o.logp[r] = 0.f;
+  if (o.wide) o.wide[r] = 0.0;
+  if (o.entropy) o.entropy[r] = 0.f;
+  if (o.state) o.state[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
 // ---- pass 1: the statistics of rows, or of parts of rows ------------------------------------------------------------------
@@ -70,15 +82,6 @@ __device__ __forceinline__ Part stream_part(const T* x, int n, float c, int t) {
   return p;
 }
 
-struct StatsOut {
-  float* logp;
-  float* entropy;
-  f32x4* state;
-  f32x4* parts;          // [rows][splits], used where splits > 1
-  RowGrad* clear;        // row gradients that a loss kernel fills in for the rows it owns
-  int again;             // a gradient pass will read the logits again
-};
-
 // One read of the logits, a running reference a thread, no more than a few floats written a row: 4096 rows of 131072 bf16 in
 // 186 us, 5.8 TB/s (a copy reaches 5.1, reading and writing); one such row, cut into 32 parts, with join_kernel in 6 us.
 template <typename T, int TPR, bool KEEP>
@@ -96,10 +99,10 @@ __global__ __launch_bounds__(NT) void stats_kernel(Logits p, int splits, int chu
     const Part q = row_join<TPR>(stream_part<T, TPR, KEEP>(x, hi - lo, p.c, t), p.c, red);     // TPR > 64: one row, so the barrier is uniform
     if (t == 0) {
       if (splits > 1) o.parts[part] = f32x4{q.m, q.s, q.w, 0.f};
-      else write_row<T>(p, r, label, q, o.logp, o.entropy, o.state);
+      else write_row<T>(p, r, label, q, o);
     }
   } else if (live && t == 0 && sp == 0) {
-    write_no_row(r, o.logp, o.entropy, o.state);
+    write_no_row(r, o);
   }
   if (live && t == 0 && sp == 0 && o.clear) o.clear[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(NT) void join_kernel(Logits p, int splits, StatsOut
     q = Part{v[0], v[1], v[2]};
   }
   q = wave_join(q, p.c);
-  if (lane == 0) write_row<T>(p, r, label, q, o.logp, o.entropy, o.state);
+  if (lane == 0) write_row<T>(p, r, label, q, o);
 }
 
 // ---- pass 2: gradient rows -----------------------------------------------------------------------------------------------
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(NT) void grad_kernel(Logits p, GradIn g, int splits
 // ---- preference loss ---------------------------------------------------------------------------------------------------
 struct PrefIn {
   Sequences seq;             // 2 P sequences: the chosen ones, then the rejected ones
-  const float* logp;
+  const double* logp;
   const f32x4* state;
   const float* ref;          // [2 P] or null
   int kind, average;
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(1024) void pref_kernel(Logits p, PrefIn q) {
     sequence(q.seq, pair + side * pairs, start[side], end[side]);
     sum[side] = n[side] = 0;
     for (unsigned r = start[side] + threadIdx.x; r < end[side]; r += blockDim.x) {
-      sum[side] += (double)q.logp[r];
+      sum[side] += q.logp[r];
       n[side] += load_index(p.labels, p.labels64, r) != p.ignore;
     }
     sum[side] = block_sum64(sum[side], red);
@@ -486,7 +489,7 @@ extern "C" size_t st_token_workspace_bytes(int dtype, long long rows, int vocab,
   if (rows < 0 || sequences < 0) return 0;
   const size_t r = (size_t)rows, q = (size_t)sequences;
   // parts, log-probabilities, statistics, pairs' losses; or rows' terms and sequences' counts
-  return std::max(parts_bytes(rows, vocab, size_of(dtype)) + align256(r * 4) + align256(r * 16) + align256(q * 8),
+  return std::max(parts_bytes(rows, vocab, size_of(dtype)) + align256(r * 8) + align256(r * 16) + align256(q * 8),
                   sums_bytes(rows) + align256(q * 4));
 }
 
@@ -543,13 +546,13 @@ extern "C" int st_preference_loss_fwd(const void* x, int dtype, long long rows, 
   StatsOut o{};
   PrefIn q{};
   o.parts = w.take<f32x4>(parts_bytes(rows, vocab, size_of(dtype)) / sizeof(f32x4));
-  o.logp = w.take<float>((size_t)rows);
+  o.wide = w.take<double>((size_t)rows);
   o.state = w.take<f32x4>((size_t)rows);
   q.each = w.take<double>((size_t)pairs);
   o.clear = reinterpret_cast<RowGrad*>(row_grad);
   o.again = row_grad != nullptr;
   q.seq = Sequences{cu_seqlens, 2u * (unsigned)pairs, (unsigned)inner, (unsigned)rows};
-  q.logp = o.logp;
+  q.logp = o.wide;
   q.state = o.state;
   q.ref = ref_logps;
   q.kind = kind;
