@@ -532,7 +532,7 @@ int st_token_loss_bwd(const void* x, int dtype, long long rows, long long inner,
  * teacher_val [rows][k]; mask [rows] (NULL: all rows) says which rows count, loss = tau^2 times their mean of
  * sum p (ln p - ln q).  tail = 0: p = softmax(val / tau) over the list.  tail = 1: p = exp(val), and what the teacher
  * and the student have off the list is one more bucket.  An index >= vocab makes its row NaN; entries with the same
- * index add up.  row_grad [rows][8] (NULL: no gradient follows). */
+ * index add up.  At most 2^20 tokens and k = 4096.  row_grad [rows][8] (NULL: no gradient follows). */
 size_t st_distill_workspace_bytes(long long rows);
 int st_distill_loss_fwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
                         long long s_inner, int vocab, const void* teacher_idx, int idx64, const float* teacher_val,

@@ -226,6 +226,7 @@ __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn
 // A row's loss (not yet times its weight) and coefficients, from the statistics off the list and the list's own sums.
 __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, const Part& off, const ListSum& o, double weight, bool repeated,
                                               f32x4& a, f32x4& b) {
+#pragma clang fp contract(off)                                  // two equal references over tau have no difference
   const Ref ref = make_ref(fmaxf(off.m, o.m), p.c), ref_off = make_ref(off.m, p.c);
   // W is not kept here (it costs a sixth of the pass over the row): what it would take out of ln S, c's rounding times the mean
   // distance from the reference, is below 1e-7, and these rows are not summed against another model's
@@ -233,16 +234,17 @@ __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, 
   rebase(s_off, unused, off.m, ref, p.c);
   rebase(s_list, unused, o.m, ref, p.c);
   const float s = s_list + s_off;
-  const double ln_z = logit_of(ref, p) + ln_wide(s);            // ln of the sum of exp(x / tau)
+  const double from = logit_of(ref, p), ln_s = ln_wide(s);      // their sum is ln of the sum of exp(x / tau); references are
+                                                                // subtracted from each other first: they may be -1e14
   const double mass = q.tail ? o.z : o.z == 0 ? 0.0 : o.z / o.z;                       // 1, or NaN
   double loss = 0;
   if (mass != 0) {
-    loss = (q.tail ? o.gap : o.gap / o.z - ln_wide((float)o.z)) + mass * (ln_z - (double)make_ref(o.m, p.c).m * p.inv_tau);
+    loss = (q.tail ? o.gap : o.gap / o.z - ln_wide((float)o.z)) + mass * (from - (double)make_ref(o.m, p.c).m * p.inv_tau + ln_s);
     if (s == 0.f) loss = INFINITY;
   }
   const double rest = q.tail && o.used < p.vocab ? (mass < 1 ? 1 - mass : mass >= 1 ? 0.0 : mass) : 0.0;
   const float inv = reciprocal(s), inv_off = reciprocal(off.s);
-  if (rest != 0) loss += off.s == 0.f ? INFINITY : rest * (ln_wide((float)rest) - (logit_of(ref_off, p) + ln_wide(off.s) - ln_z));
+  if (rest != 0) loss += off.s == 0.f ? INFINITY : rest * (ln_wide((float)rest) - (logit_of(ref_off, p) - from + (ln_wide(off.s) - ln_s)));
   const double gr = q.scale * weight * p.tau, total = mass + rest;
   const float on = s == 0.f ? 0.f : (float)(gr * total * (double)inv);
   const double back = (double)__builtin_amdgcn_exp2f(step(off.m, ref, p.c));

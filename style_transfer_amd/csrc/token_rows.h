@@ -15,9 +15,9 @@
 // multiplied by a power of two, exactly.  (The hardware's exponential is 3.4e-9 too small on average, and an element would go
 // through four of them on its way into S.)
 //
-// Where |m c| reaches 1e30 ("low" rows: nothing but the lowest value of the type, as a mask leaves them) the difference comes
-// first, d_j = (x_j - m) c, which cannot overflow against itself: such a row is the uniform distribution that the formula
-// gives.  A row of -inf only has S = 0: no distribution, log-probability -inf, entropy 0, gradient 0.
+// Where |m c| reaches 2^24 ("low" rows: nothing but a mask's value, -1e9 or the lowest of the type) the next whole number can be
+// far from it, and the difference comes first, d_j = (x_j - m) c: such a row is the uniform distribution that the formula gives,
+// whatever the value.  A row of -inf only has S = 0: no distribution, log-probability -inf, entropy 0, gradient 0.
 //
 // Sums of a row are fp32 per thread and over a fixed tree; what a row is reduced to is finished around fp64 sums (one wave a
 // row), because a sequence's sum of hundreds of log-probabilities is compared with another model's: c's own rounding
@@ -118,9 +118,9 @@ struct Part {
   float m, s, w;
 };
 
-constexpr float LOW = 1e30f, FAR = 0x1p80f;
+constexpr float LOW = 0x1p24f, FAR = 0x1p80f;
 
-// A reference and its product with c as a whole number (above 2^23 every float is one).
+// A reference and its product with c as a whole number.
 struct Ref {
   float m, mc;
   bool low;
@@ -313,8 +313,9 @@ __device__ __forceinline__ RowStat finish(const Part& q, const Logits& p) {
   return r;
 }
 
-// natural logarithm of q at a logit
+// natural logarithm of q at a logit (not fused: what the reference itself is over tau leaves nothing)
 __device__ __forceinline__ double log_prob(float x, const RowStat& r, const Logits& p) {
+#pragma clang fp contract(off)
   return r.inv_ts == 0.f ? -INFINITY : (double)x * p.inv_tau - r.z - r.ln_s;
 }
 

@@ -611,6 +611,38 @@ def test_low_logits_behind_masked_ones(dtype, vocab):
         close(leaf.grad, want, distill_bound(x, idx, val, None, 1.0, want, dtype), "distillation gradient")
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1000), (torch.bfloat16, 5001), (torch.float32, 20000), (torch.bfloat16, 140000)])
+@pytest.mark.parametrize("value", [-2e7, -1e9, -1e10, -3e14, -1e29, 5e10])
+def test_rows_of_a_finite_mask(dtype, vocab, value):
+    """Rows that hold nothing but a mask's value, or a second one far below it: uniform over the largest, whatever its size."""
+    from style_transfer_amd.losses import clipped_policy_loss, topk_distill_loss, token_logprobs
+    x = torch.full((3, vocab), value).to(dtype)
+    x[1, vocab // 2:] = -math.inf
+    x[2, : vocab // 3] = torch.tensor(value).to(dtype) - abs(value) / 8
+    t = torch.tensor([vocab - 1, 3, vocab // 2])
+    for tau in (1.0, 0.7):
+        logp, h, log_q, q = O.token_logprobs(x, t, tau)
+        leaf = x.cuda().requires_grad_(True)
+        got, entropy = token_logprobs(leaf, t.cuda(), temperature=tau, return_entropy=True)
+        close(got, logp, row_error(vocab) + logp.abs() * 2 * U, "logp")
+        close(entropy, h, (h + 2) * row_error(vocab) + 2 * h * U, "entropy")
+        loss, stats, want = O.policy(x, t, [(0, 3)], logp.float(), torch.ones(3), ent=0.1, tau=tau)
+        policy = clipped_policy_loss(leaf[None], t[None].cuda(), logp.float()[None].cuda(), torch.ones(1, 3).cuda(), entropy_coef=0.1, temperature=tau)
+        policy.loss.backward()
+        err = row_error(vocab) + 24 * U
+        close(policy.stats, stats, 14 * err + stats.abs() * 2 * U, "stats")
+        third = torch.full((3,), 1 / 3, dtype=torch.float64)
+        close(leaf.grad, want, grad_bound(want, dtype, log_q, third, third / 10, h, tau, extra=2 * err), "policy gradient")
+        idx, val = torch.tensor([[1, 2], [3, 4], [vocab - 1, vocab - 2]]), torch.tensor([[-0.5, -1.5]]).repeat(3, 1)
+        for tail in (False, True):
+            loss, want = O.distill(x, idx, val, None, tau, tail)
+            leaf.grad = None
+            got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), temperature=tau, tail=tail)
+            got.backward()
+            close(got, torch.tensor(loss), 2 * row_error(vocab) + 60 * U + abs(loss) * 8 * U, "loss")
+            close(leaf.grad, want, distill_bound(x, idx, val, None, tau, want, dtype), "distillation gradient")
+
+
 def test_a_padded_batch_in_place():
     """Rows of a slice at every alignment through the kernels that hold a row: as of a copy, and no other memory is written."""
     from style_transfer_amd import losses
@@ -823,6 +855,21 @@ def test_logits_kept_elsewhere_until_the_backward(vocab):
                 del other
             half = 2 * row_error(vocab)
             assert torch.allclose(grads[0], grads[1], rtol=half, atol=half * float(grads[0].abs().max()))
+
+
+def test_inside_a_checkpoint():
+    """Recomputed in the backward pass, as memory-saving training does: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    x, t, idx, val = batch(7, 5000)
+    from style_transfer_amd import losses
+    old = losses.token_logprobs(x, t) + 0.1
+    grads = []
+    for saving in (False, True):
+        leaf = x.clone().requires_grad_(True)
+        step = lambda v: all_losses(v * 1.5, t, idx, val, old, old - 0.2)  # noqa: E731
+        (checkpoint(step, leaf, use_reentrant=False) if saving else step(leaf)).backward()
+        grads.append(leaf.grad)
+    assert torch.equal(*grads)
 
 
 def test_a_changed_input_is_noticed():
