@@ -611,6 +611,33 @@ def test_low_logits_behind_masked_ones(dtype, vocab):
         close(leaf.grad, want, distill_bound(x, idx, val, None, 1.0, want, dtype), "distillation gradient")
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 2 ** 20), (torch.bfloat16, 2 ** 20), (torch.float16, 2 ** 19 + 3), (torch.float32, 400003)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_the_largest_vocabularies(dtype, vocab, tail):
+    from style_transfer_amd.losses import clipped_policy_loss, topk_distill_loss
+    n, k = 3, 40
+    x = logits(n, vocab, dtype, vocab)
+    idx, val = teacher(x, k, 1.0, tail, 2)
+    idx[:, 0], idx[0, 1] = vocab - 1, 0
+    loss, want = O.distill(x, idx, val, None, 1.0, tail)
+    wide = torch.zeros(n, vocab + 3, dtype=dtype)
+    wide[:, 3:] = x                                             # no row begins on 16 bytes
+    leaf = wide.cuda()[:, 3:].requires_grad_(True)
+    got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)
+    got.backward()
+    close(got, torch.tensor(loss), 2 * row_error(vocab) + 60 * U + abs(loss) * 4 * U, "loss")
+    close(leaf.grad, want, distill_bound(x, idx, val, None, 1.0, want, dtype), "gradient")
+    t = torch.tensor([vocab - 1, 0, 77])
+    logp, h, log_q, q = O.token_logprobs(x, t)
+    loss, stats, want = O.policy(x, t, [(0, n)], logp.float(), torch.ones(n))
+    leaf.grad = None
+    got = clipped_policy_loss(leaf[None], t[None].cuda(), logp.float()[None].cuda(), torch.ones(1, n).cuda())
+    got.loss.backward()
+    err = row_error(vocab) + 40 * U
+    close(got.stats, stats, 20 * err + stats.abs() * 2 * U, "stats")
+    close(leaf.grad, want, grad_bound(want, dtype, log_q, torch.full((n,), 1 / n, dtype=torch.float64), extra=2 * err), "policy gradient")
+
+
 @pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1000), (torch.bfloat16, 5001), (torch.float32, 20000), (torch.bfloat16, 140000)])
 @pytest.mark.parametrize("value", [-2e7, -1e9, -1e10, -3e14, -1e29, 5e10])
 def test_rows_of_a_finite_mask(dtype, vocab, value):
