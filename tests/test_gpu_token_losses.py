@@ -899,6 +899,23 @@ def test_inside_a_checkpoint():
     assert torch.equal(*grads)
 
 
+def test_no_second_derivative():
+    """A graph of the gradient can be asked for; going through it is refused, not answered with 0."""
+    from style_transfer_amd import losses
+    x, t, idx, val = batch(9)
+    old = losses.token_logprobs(x, t)
+    for fn in (lambda v: losses.token_logprobs(v, t).sum(), lambda v: losses.preference_loss(v, t).loss,
+               lambda v: losses.clipped_policy_loss(v, t, old, old + 9).loss, lambda v: losses.topk_distill_loss(v, idx, val, tail=True)):
+        leaf = x.clone().requires_grad_(True)
+        plain, = torch.autograd.grad(fn(leaf), [leaf])
+        weight = torch.ones((), device="cuda", requires_grad=True)
+        for loss, why in ((fn(leaf), "does not require grad"), (weight * fn(leaf), "once_differentiable")):
+            grad, = torch.autograd.grad(loss, [leaf], create_graph=True)
+            assert torch.equal(grad.detach(), plain)
+            with pytest.raises(RuntimeError, match=why):
+                grad.sum().backward()
+
+
 def test_a_changed_input_is_noticed():
     from style_transfer_amd import losses
     x, t, _, _ = batch(8)
