@@ -418,12 +418,13 @@ struct Split {
   int tpr, splits, chunk;
 };
 
-// Threads of a part and parts of a row.  A row of up to 4 KB is a wave's work (four rows a block share no barrier); a
-// longer one is a block's.  Where the rows alone would leave compute units idle, a row is cut until there are about four
+// Threads of a part and parts of a row.  A row of up to 4 KB is a wave's work (four rows a block share no barrier), and one of up
+// to 32 KB where there are enough rows to fill the compute units with waves (forward, bf16: 16384 x 4096 37 -> 26 us, 10300 x
+// 6618 37 -> 27, 2048 x 16380 16.7 -> 15.3; 1024 x 8190 7.0 against 7.5, 8192 x 32768 97 against 105); a longer one is a block's.  Where the rows alone would leave compute units idle, a row is cut until there are about four
 // blocks for each of the 256, in parts of 8 KB at least (two 16-byte loads a thread).
 Split split_of(unsigned rows, int vocab, int size) {
   const long long bytes = (long long)vocab * size;
-  if (bytes <= 4096) return {64, 1, vocab};
+  if (bytes <= 4096 || (bytes <= 32768 && rows >= 2048)) return {64, 1, vocab};
   int s = 1;
   if (rows < 1024) s = (int)std::min<long long>(MAX_SPLITS, std::min(st::cdivll(1024, std::max(1u, rows)), bytes / 8192));
   s = std::max(1, s);
@@ -458,10 +459,11 @@ int launch_stats(const char* who, int dtype, const Logits& p, const StatsOut& o,
 
 template <typename T>
 int launch_grad_t(const char* who, const Logits& p, const GradIn& g, void* grad, hipStream_t s) {
-  // parts of 16 KB: four 16-byte loads a thread, and enough blocks whatever the number of rows
+  // parts of 16 KB: four 16-byte loads a thread, and enough blocks whatever the number of rows; rows of up to 8 KB are a wave's
+  // (16384 x 2500 bf16: 29 us against 33; of 13 KB, 10300 x 6618: 54 against 47)
   const long long bytes = (long long)p.vocab * (long long)sizeof(T);
-  const int tpr = bytes <= 4096 ? 64 : NT;
-  const int chunk = bytes <= 4096 ? p.vocab : 16384 / (int)sizeof(T);
+  const int tpr = bytes <= 8192 ? 64 : NT;
+  const int chunk = bytes <= 8192 ? p.vocab : 16384 / (int)sizeof(T);
   const int splits = (int)st::cdivll(p.vocab, chunk);
   // a launch that may have nothing to do is kept small: 131072 blocks that end at once take 28 us, 4096 take 3
   const long long blocks = std::min<long long>(st::cdivll((long long)p.rows * splits, NT / tpr), g.skip_if_one ? 4096 : 1LL << 23);

@@ -143,6 +143,37 @@ def test_masked_logits_and_empty_rows(dtype, vocab):
     assert not leaf.grad[3:6].any() and torch.isnan(leaf.grad[6:]).all()
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1030), (torch.bfloat16, 4097), (torch.float16, 8000), (torch.bfloat16, 16383), (torch.float32, 8193)])
+def test_many_rows_of_middle_size(dtype, vocab):
+    """From 2048 rows on a row of up to 32 KB is a wave's: the same as of fewer rows at a time, and as the formula."""
+    from style_transfer_amd.losses import token_logprobs
+    rows = 2050
+    x, t = logits(40, vocab, dtype, vocab).repeat(rows // 40 + 1, 1)[:rows], labels_for(rows, vocab, 3)
+    x[1::40, : vocab // 2] = -math.inf
+    t[t >= 0] = t[t >= 0] // 2 + vocab // 2                     # not a masked one
+    leaf = x.cuda().requires_grad_(True)
+    got, h = token_logprobs(leaf, t.cuda(), temperature=0.9, return_entropy=True)
+    w = rand(4, rows).cuda()
+    (got * w + h).sum().backward()
+    few = x.cuda().requires_grad_(True)
+    for part in range(0, rows, 1025):
+        a, b = token_logprobs(few[part:part + 1025], t[part:part + 1025].cuda(), temperature=0.9, return_entropy=True)
+        err = row_error(vocab)
+        assert torch.allclose(got[part:part + 1025], a, atol=2 * err, rtol=4 * U) and torch.allclose(h[part:part + 1025], b, atol=24 * err, rtol=4 * U)
+        (a * w[part:part + 1025] + b).sum().backward()
+    # per unit of a probability: the row's error times what multiplies it, |w| + |log q| + h
+    half, tiny = HALF[dtype]
+    size = 2 * row_error(vocab) * (float(w.abs().max()) + 40)
+    assert torch.allclose(leaf.grad.float(), few.grad.float(), rtol=2 * half, atol=size + tiny)
+    some = slice(0, 44)
+    logp, entropy, log_q, q = O.token_logprobs(x[some], t[some], 0.9)
+    close(got[some], logp, row_error(vocab) + logp.abs() * 2 * U, "logp")
+    close(h[some], entropy, (entropy + 2) * row_error(vocab) + 2 * entropy * U, "entropy")
+    a, b = w[some].cpu().double(), torch.ones(44, dtype=torch.float64)
+    want = O.row_gradient(t[some], 0.9, entropy, log_q, q, a, b)
+    close(leaf.grad[some], want, grad_bound(want, dtype, log_q, a, b, entropy, 0.9), "gradient")
+
+
 def test_labels_outside_the_vocabulary_are_nan_and_touch_nothing():
     from style_transfer_amd.losses import token_logprobs
     x = logits(4, 130, torch.float32, 5)
