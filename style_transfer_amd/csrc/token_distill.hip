@@ -294,7 +294,7 @@ __global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, S
   __shared__ f32x4 told[2];
   const int t = threadIdx.x % TPR;
   const M marks{all_bits + (threadIdx.x / TPR) * words};
-  const unsigned r = blockIdx.x * S::ROWS + threadIdx.x / TPR;
+  const unsigned r = blockIdx.x * S::ROWS + (S::ROWS > 1 ? scalar(threadIdx.x / TPR) : 0);      // the same for a wave
   const bool counts = r < p.rows && (!q.mask || q.mask[r]);
   if (!counts) {                                                // all threads of the row
     if (r >= p.rows) return;

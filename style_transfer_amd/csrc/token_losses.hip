@@ -88,7 +88,7 @@ template <typename T, int TPR, bool KEEP>
 __global__ __launch_bounds__(NT) void stats_kernel(Logits p, int splits, int chunk, StatsOut o) {
   __shared__ Part red[NT / 64];
   const int t = threadIdx.x % TPR;
-  const unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const unsigned long long part = (unsigned long long)blockIdx.x * (NT / TPR) + scalar(threadIdx.x / TPR);    // the same for a wave
   const unsigned r = (unsigned)(part / splits);
   const int sp = (int)(part % splits);
   const bool live = r < p.rows;
@@ -357,14 +357,15 @@ __global__ __launch_bounds__(1024) void count_kernel(Logits p, PolicyIn q, Sums 
 // One pass: a row's statistics, its terms and, where the caller wants one, its gradient (for an upstream gradient of 1).  With
 // the row in registers the logits are read once: 4096 rows of 131072 bf16 in 415 us, 5.2 TB/s read and written (two passes would take
 // 552), of 32768 in 101 us, 5.3 TB/s; 1024 rows of 131072 fp32, of which the last 192 KB each are read twice, in 237 us, 4.5 TB/s.
-// Rows of 2 KB are bound by what a wave does once a row (65536 of 1000 bf16: 78 us, 3.4 TB/s).
+// Rows of 2 KB are bound by what a wave does once a row (65536 of 1000 bf16: 73 us, 3.6 TB/s; 78 before the row's number was in a
+// scalar register).
 template <typename T, typename S>
 __global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, Sums u, T* __restrict__ grad) {
   constexpr int TPR = S::TPR;
   __shared__ Part red[TPR / 64];
   __shared__ f32x4 told;
   const int t = threadIdx.x % TPR;
-  const unsigned r = blockIdx.x * S::ROWS + threadIdx.x / TPR;
+  const unsigned r = blockIdx.x * S::ROWS + (S::ROWS > 1 ? scalar(threadIdx.x / TPR) : 0);      // the same for a wave
   if (r >= p.rows) return;                                      // whole waves (TPR = 64) or the whole block
   const long long label = load_index(p.labels, p.labels64, r);
   const int s = sequence_of(q.seq, r);
