@@ -285,7 +285,7 @@ __device__ __forceinline__ bool sync_row_or(bool v) {
 // reaches); of 131072 in 463 us, 4.6 TB/s, where one row fills a compute unit and its reading and writing take turns; 1024 rows of
 // 131072 fp32, of which the last 192 KB each are read twice, in 242 us, 4.4 TB/s.
 template <typename T, typename S>
-__global__ __launch_bounds__(S::BLOCK) void distill_kernel(Logits p, ListIn q, Sums u, int words, T* __restrict__ grad) {
+__global__ __launch_bounds__(S::BLOCK, 4) void distill_kernel(Logits p, ListIn q, Sums u, int words, T* __restrict__ grad) {
   constexpr int TPR = S::TPR, VEC = Type<T>::VEC;
   using M = Marks<T, TPR>;
   extern __shared__ uint32_t all_bits[];

@@ -360,7 +360,7 @@ __global__ __launch_bounds__(1024) void count_kernel(Logits p, PolicyIn q, Sums 
 // Rows of 2 KB are bound by what a wave does once a row (65536 of 1000 bf16: 73 us, 3.6 TB/s; 78 before the row's number was in a
 // scalar register).
 template <typename T, typename S>
-__global__ __launch_bounds__(S::BLOCK) void policy_kernel(Logits p, PolicyIn q, Sums u, T* __restrict__ grad) {
+__global__ __launch_bounds__(S::BLOCK, 4) void policy_kernel(Logits p, PolicyIn q, Sums u, T* __restrict__ grad) {
   constexpr int TPR = S::TPR;
   __shared__ Part red[TPR / 64];
   __shared__ f32x4 told;

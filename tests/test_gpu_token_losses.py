@@ -558,6 +558,9 @@ def far_logits(n, vocab, dtype, seed):
     return x
 
 
+SIZES += [(torch.bfloat16, 70001), (torch.float32, 40960), (torch.float16, 81921)]       # 140 KB, 160 KB and a little more
+
+
 @pytest.mark.parametrize("dtype,vocab", SIZES)
 def test_policy_rows_of_every_size(dtype, vocab):
     from style_transfer_amd.losses import clipped_policy_loss
