@@ -67,7 +67,7 @@ def preference(x, labels, seqs, ref=None, beta=0.1, kind="sigmoid", smoothing=0.
         if kind == "sigmoid":
             soft = lambda v: max(v, 0.0) + math.log1p(math.exp(-abs(v)))  # noqa: E731
             sig = lambda v: 1 / (1 + math.exp(-v)) if v > -700 else 0.0  # noqa: E731
-            loss += (1 - smoothing) * soft(-z) + smoothing * soft(z)
+            loss += (1 - smoothing) * soft(-z) + (smoothing * soft(z) if smoothing else 0.0)      # z may be +inf
             slope = beta * (smoothing * sig(z) - (1 - smoothing) * sig(-z))
         elif kind == "ipo":
             loss += (gap - 0.5 / beta) ** 2

@@ -223,7 +223,8 @@ __global__ __launch_bounds__(1024) void pref_kernel(Logits p, PrefIn q) {
     double loss, slope;
     if (q.kind == ST_PREF_SIGMOID) {
       const double e = exp(-fabs(z)), soft = log1p(e), small = e / (1 + e), large = 1 / (1 + e);
-      loss = (1 - q.smoothing) * (soft + fmax(-z, 0.0)) + q.smoothing * (soft + fmax(z, 0.0));
+      loss = (1 - q.smoothing) * (soft + fmax(-z, 0.0));
+      if (q.smoothing != 0) loss += q.smoothing * (soft + fmax(z, 0.0));       // z is +inf where a rejected label is masked
       slope = q.beta * (q.smoothing * (z > 0 ? large : small) - (1 - q.smoothing) * (z > 0 ? small : large));
       if (z != z) loss = slope = z;
     } else if (q.kind == ST_PREF_IPO) {
