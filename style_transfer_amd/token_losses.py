@@ -15,6 +15,7 @@ What they have in common:
   ``[T, V]`` logits; rows outside all of them do not count and get a zero gradient.
 * With nothing that counts a loss is 0.  ``scale`` multiplies a loss and its gradient (a weight, 1 / accumulation steps, a
   static loss scale).
+* Derivatives are reverse-mode and of first order: a forward-mode tangent or a second derivative is refused.
 * Results do not depend on the run: every sum has a fixed order.
 * ``clipped_policy_loss`` and ``topk_distill_loss`` write the gradient of logits that require one in the forward pass, while
   a row is on chip.  A backward pass with an upstream gradient of 1 hands it over; another one (a loss weight outside, a
@@ -27,6 +28,7 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -232,7 +234,8 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
 
 
 def _wants_grad(x: torch.Tensor) -> bool:
-    return x.requires_grad and torch.is_grad_enabled()
+    # a forward-mode tangent: the autograd function refuses it; without one the result would carry none, a derivative of 0
+    return (x.requires_grad and torch.is_grad_enabled()) or fwAD.unpack_dual(x).tangent is not None
 
 
 # ---- the two losses whose rows go through the label's log-probability -------------------------------------------------------------
