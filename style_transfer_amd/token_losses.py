@@ -247,6 +247,8 @@ def _take_grad(ctx, x):
 
 
 def _token_loss_bwd(ctx, gout):
+    if gout is None:                                           # a node above has none for the loss
+        return None, None
     x, labels, row_grad = ctx.saved_tensors
     args, tau, ignore = ctx.call
     grad, for_one = _take_grad(ctx, x)

@@ -61,3 +61,23 @@ def test_forward_mode_derivatives_are_refused(nothing_runs, name, mode):
         assert not CALLS[name](losses, X).requires_grad         # without a tangent a level changes nothing
         with pytest.raises(NotImplementedError):
             CALLS[name](losses, fwAD.make_dual(X, torch.ones_like(X)))
+
+
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a):
+        return a.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_loss_without_an_upstream_gradient(nothing_runs, name):
+    """A node above whose backward gives None: nothing comes from there, and what else reaches the logits does."""
+    from style_transfer_amd import losses
+    leaf = X.clone().requires_grad_(True)
+    (_NoGradient.apply(CALLS[name](losses, leaf * 1)) + leaf.sum()).backward()
+    if name != "topk_distill_loss":                             # its kernel gets a gradient of 0, and is not there
+        assert torch.equal(leaf.grad, torch.ones_like(X))
