@@ -94,11 +94,10 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
   for (int i = k;;) {
     if (e.j >= 0) {
       const float d = distance((float)e.x, ref, p.c), ex = __builtin_amdgcn_exp2f(d);
-      const double lv = ((double)e.v - from) * it;
-      const float ev = exp_wide(lv);
+      const double lv = ((double)e.v - from) * it, ev = exp64(lv);      // 64 bits: 1 - sum p has no digit left of a p rounded to 32
       s += ex;
-      z += (double)ev;
-      if (ev != 0.f) gap += (double)ev * (lv - ((double)(float)e.x - (double)ref.m) * p.inv_tau);
+      z += ev;
+      if (ev != 0.0) gap += ev * (lv - ((double)(float)e.x - (double)ref.m) * p.inv_tau);
     }
     if ((i += threads) >= q.k) break;
     e = load_entry(p, q, r, i, x);
@@ -121,7 +120,7 @@ __device__ __forceinline__ ListSum join_lists(const Logits& p, const ListIn& q, 
   const bool any = part.z != 0;
   const double a = !any || q.tail ? 0.0 : ((double)part.vref - (double)o.vref) * p.inv_tau;
   const double b = any && part.m > -INFINITY ? ((double)part.m - (double)ref.m) * p.inv_tau : 0.0;
-  const double f = any ? (double)exp_wide(a) : 0.0;
+  const double f = any ? exp64(a) : 0.0;
   o.s = lanes_sum<16>(s);
   o.z = lanes_sum(any ? f * part.z : 0.0);
   o.gap = lanes_sum(any ? f * (part.gap + part.z * (a - b)) : 0.0);

@@ -58,3 +58,32 @@ def test_the_smoothed_part_of_an_infinite_difference(smoothing):
     assert float(loss) == (INF if smoothing else 0.0)
     loss = preference_loss(x.flip(0).cuda(), t.cuda(), label_smoothing=smoothing).loss
     assert float(loss) == INF
+
+
+# ---- distillation: what a confident teacher leaves for the rest -----------------------------------------------------------------
+@pytest.mark.parametrize("vocab", [1000, 20000])
+@pytest.mark.parametrize("k,left", [(1, 1e-5), (1, 1e-6), (64, 1e-4), (64, 1e-5), (64, 1e-6)])
+def test_distill_teacher_that_leaves_next_to_nothing(vocab, k, left):
+    """1 - sum p where p was stored as fp32 log-probabilities: they hold the digits, and an entry's own rounding may not take them.
+    The student leaves a tenth of that off the list, so that the rest decides the gradient there."""
+    from style_transfer_amd.losses import topk_distill_loss
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(3, vocab, generator=g)
+    idx = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(3)])
+    x.scatter_(1, idx, x.gather(1, idx) + math.log(vocab / k) + math.log(10 / left))
+    val = (torch.log_softmax(torch.randn(3, k, generator=g, dtype=torch.float64), 1) + math.log1p(-left)).float()
+    loss, want = O.distill(x, idx, val, None, 1.0, True)
+    leaf = x.cuda().requires_grad_(True)
+    got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=True)
+    got.backward()
+    # off the list an entry is q_j - rest e_j / S_off, over the rows: q_j and e_j / S_off have a row's error R each (sums of V terms,
+    # the exponential's argument of up to 40 bits), rest the fp64 sum's, K 2^-46 / left, which is nothing.  With r = rest / q_rest
+    # that is R (1 + r) of the |1 - r| q_j that are left, and a few roundings.
+    off = torch.ones(3, vocab, dtype=torch.bool).scatter_(1, idx, False)
+    grad = leaf.grad.cpu().double()
+    q_rest = torch.stack([O.row(r, 1.0)[1] for r in x]).mul(off).sum(1)
+    r = ((1 - val.double().exp().sum(1)) / q_rest)[:, None]
+    bound = want.abs() * ((vocab / 64 + 64 + 80) * (1 + r) / (1 - r).abs() + 20) * U
+    assert float(r.max()) > 1 and bool(((grad - want).abs() <= bound)[off].all())
+    # a listed entry p_k (log p_k - log q_k) has a row's error, the rest's term next to none
+    assert abs(float(got.detach()) - loss) <= (vocab / 64 + 64 + 80) * U
