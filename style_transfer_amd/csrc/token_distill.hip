@@ -123,7 +123,7 @@ __device__ __forceinline__ ListSum join_lists(const Logits& p, const ListIn& q, 
   const double f = any ? exp64(a) : 0.0;
   o.s = lanes_sum<16>(s);
   o.z = lanes_sum(any ? f * part.z : 0.0);
-  o.gap = lanes_sum(any ? f * (part.gap + part.z * (a - b)) : 0.0);
+  o.gap = lanes_sum(f != 0.0 ? f * (part.gap + part.z * (a - b)) : 0.0);      // an entry without mass does not count: its logit may be -inf
   o.used = (int)lanes_sum<16>((float)part.used);
   o.bad = __any(part.bad);
   return o;

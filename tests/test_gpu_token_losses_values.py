@@ -87,3 +87,32 @@ def test_distill_teacher_that_leaves_next_to_nothing(vocab, k, left):
     assert float(r.max()) > 1 and bool(((grad - want).abs() <= bound)[off].all())
     # a listed entry p_k (log p_k - log q_k) has a row's error, the rest's term next to none
     assert abs(float(got.detach()) - loss) <= (vocab / 64 + 64 + 80) * U
+
+
+# ---- distillation: entries without any mass ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("vocab,k", [(9000, 128), (20000, 300), (131072, 2000)])
+@pytest.mark.parametrize("value", [-1e9, -300.0, torch.finfo(torch.float32).min])
+def test_distill_entries_that_both_models_mask(vocab, k, tail, value):
+    """A list filled up with masked tokens: the teacher's values are a mask's, the student's logits -inf.  Where they have no mass in 64
+    bits, what the student says of them does not count, whichever wave they are in; exp(-300) is a mass that the student denies."""
+    from style_transfer_amd.losses import topk_distill_loss
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(2, vocab, generator=g)
+    idx = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(2)])
+    val = torch.log_softmax(torch.randn(2, k, generator=g), 1) - 0.2
+    x[0].index_fill_(0, idx[0, 40:], -INF)                      # all behind the first 40; a few in the middle
+    val[0, 40:] = value
+    x[1].index_fill_(0, idx[1, 5:9], -INF)
+    val[1, 5:9] = value
+    loss, want = O.distill(x, idx, val, None, 1.0, tail)
+    assert math.isfinite(loss) == (value != -300)
+    leaf = x.cuda().requires_grad_(True)
+    got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)
+    got.backward()
+    row = (vocab / 64 + 64) * U
+    bound = 2 * row + 60 * U + k / 16 * U + abs(loss) * 4 * U
+    assert float(got.detach()) == loss if math.isinf(loss) else abs(float(got.detach()) - loss) <= bound
+    # rows are halved by the mean: an entry q_j Q - p_j, each with a row's error and 40 bits of its exponent
+    grad = leaf.grad.cpu().double()
+    assert bool(((grad - want).abs() <= (2 * row + k / 16 * U + 200 * U) * (want.abs() + 2e-4) + 2.0 ** -126).all())
