@@ -136,9 +136,13 @@ __device__ __forceinline__ float distance(float x, const Ref& r, float c) {
 }
 __device__ __forceinline__ float distance(float x, const Ref& r, float c) { return r.low ? distance<true>(x, r, c) : distance<false>(x, r, c); }
 
-// from an old reference to a new one; -inf where the old part is empty
+// From an old reference to a new one; -inf where the old part is empty.  One of them may be low and the other not: the whole
+// number is the reference then, not the m that it came from, which is up to half a bit away.
 __device__ __forceinline__ float step(float m_old, const Ref& to, float c) {
-  return to.low ? (m_old - to.m) * c : rintf(m_old * c) - to.mc;
+  if (m_old == -INFINITY) return -INFINITY;
+  const Ref from = make_ref(m_old, c);
+  if (from.low) return distance(m_old, to, c);
+  return to.low ? -fmaf(to.m, c, -from.mc) : from.mc - to.mc;
 }
 
 // A part seen from another reference: d' = d + t.

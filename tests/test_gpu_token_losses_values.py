@@ -116,3 +116,30 @@ def test_distill_entries_that_both_models_mask(vocab, k, tail, value):
     # rows are halved by the mean: an entry q_j Q - p_j, each with a row's error and 40 bits of its exponent
     grad = leaf.grad.cpu().double()
     assert bool(((grad - want).abs() <= (2 * row + k / 16 * U + 200 * U) * (want.abs() + 2e-4) + 2.0 ** -126).all())
+
+
+# ---- references on both sides of 2^24 ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("vocab", [1000, 20000, 131072])
+def test_parts_whose_references_lie_on_both_sides_of_a_border(vocab, sign):
+    """Up to |m c| < 2^24 a reference is the whole number next to m c, beyond it m itself: a part of each kind, one unit of the
+    last place apart in x, joins without the up to half a bit between the two readings."""
+    from style_transfer_amd.losses import token_logprobs, topk_distill_loss
+    x = torch.full((2, vocab), sign * 11629077.0)               # x c = 16777211.49
+    x[:, vocab // 2:] = sign * 11629080.0                       # 16777215.82, which is 2^24 in fp32
+    x[1] = x[1].flip(0)
+    t = torch.tensor([0, 0])
+    logp, h, log_q, q = O.token_logprobs(x, t)
+    got, entropy = token_logprobs(x.cuda(), t.cuda(), return_entropy=True)
+    row = (vocab / 64 + 64) * U
+    assert float((got.cpu().double() - logp).abs().max()) <= row + 2 * U * float(logp.abs().max())
+    assert float((entropy.cpu().double() - h).abs().max()) <= (float(h.max()) + 2) * row + 2 * U * float(h.max())
+    idx = torch.tensor([[0, 1], [vocab - 1, vocab - 2]])        # the list on one side of the border, most of the row on the other
+    val = torch.tensor([[-0.5, -1.5]]).repeat(2, 1)
+    for tail in (False, True):
+        loss, want = O.distill(x, idx, val, None, 1.0, tail)
+        leaf = x.cuda().requires_grad_(True)
+        got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)
+        got.backward()
+        assert abs(float(got.detach()) - loss) <= 2 * row + 60 * U + abs(loss) * 8 * U
+        assert bool(((leaf.grad.cpu().double() - want).abs() <= (2 * row + 60 * U) * (want.abs() + 2 / vocab)).all())
