@@ -128,6 +128,8 @@ def distill(x, idx, val, mask=None, tau=1.0, tail=False):
         if any(j >= vocab for j, _ in used):
             total, grad[r] = math.nan, math.nan
             continue
+        if not used:
+            continue
         if tail:
             log_p = [v for _, v in used]
         else:

@@ -249,6 +249,10 @@ __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, 
   const double back = (double)__builtin_amdgcn_exp2f(step(off.m, ref, p.c));
   a = f32x4{ref_off.m, s == 0.f || off.s == 0.f ? 0.f : (float)(gr * (total * (double)inv * back - rest * (double)inv_off)), ref.m, on};
   b = f32x4{o.vref == -INFINITY ? 0.f : o.vref, s == 0.f || mass == 0 ? 0.f : (float)(q.tail ? gr : gr / o.z), repeated ? 1.f : 0.f, s == 0.f || total == 0 ? 0.f : 1.f};
+  if (o.used == 0) {                                            // nothing is listed: nothing to learn, whatever the logits hold
+    loss = 0;
+    a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   if (o.bad) {
     loss = NAN;
     a[1] = a[3] = NAN;

@@ -143,3 +143,24 @@ def test_parts_whose_references_lie_on_both_sides_of_a_border(vocab, sign):
         got.backward()
         assert abs(float(got.detach()) - loss) <= 2 * row + 60 * U + abs(loss) * 8 * U
         assert bool(((leaf.grad.cpu().double() - want).abs() <= (2 * row + 60 * U) * (want.abs() + 2 / vocab)).all())
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("vocab", [300, 9000])
+def test_distill_a_position_without_entries_contributes_nothing(vocab, tail):
+    """Whatever its logits hold: a row of -inf, one with an infinity or a NaN, an ordinary one.  It counts in the mean."""
+    from style_transfer_amd.losses import topk_distill_loss
+    x = torch.randn(5, vocab, generator=torch.Generator().manual_seed(2))
+    x[1] = -INF
+    x[2, 7] = INF
+    x[3, 8] = math.nan
+    idx, val = torch.full((5, 3), -1), torch.zeros(5, 3)
+    idx[4], val[4] = torch.tensor([1, 2, 5]), torch.tensor([-1.0, -1.5, -2.0])
+    loss, want = O.distill(x[4:], idx[4:], val[4:], None, 1.0, tail)
+    leaf = x.cuda().requires_grad_(True)
+    got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)
+    got.backward()
+    assert abs(float(got.detach()) - loss / 5) <= (2 * (vocab / 64 + 64) + 60) * U
+    assert not leaf.grad[:4].any() and leaf.grad[4].any()
+    (2 * topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)).backward()      # computed again
+    assert not leaf.grad[:4].any()
