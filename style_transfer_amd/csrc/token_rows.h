@@ -8,11 +8,12 @@
 // Every loss here reaches x through the label's log-probability and the entropy, or through a short list of entries, so
 // every gradient row is   g_j = (alpha + gamma d_j) e_j   plus a few patched entries.
 //
-// m is any value near the maximum, not the maximum itself: a wave takes the largest of its first vectors, and where the rest
-// of the row lies so far above it that S leaves 2^80 it starts again with the maximum.  That saves a pass over the row, and
-// lets the exponentials begin while the row is still arriving.  m c is rounded to a whole number, which then stands for the
-// reference everywhere: d_j is one fused multiply-add with no error but its own, and a part seen from another reference is
-// multiplied by a power of two, exactly.  (The hardware's exponential is 3.4e-9 too small on average, and an element would go
+// m is a value near the maximum, not the maximum itself: a wave takes the largest of its first vector and another one where an
+// element lies more than a bit above it.  That saves a pass over the row, and lets the exponentials begin while the row is
+// still arriving; and since no d_j is above 1.5, the elements that S consists of have an exponent without error.  (With the
+// first reference kept as long as S stays below 2^80 a dominant element's d_j reaches 80, whose rounding is 2.6e-6 of S.)  m c
+// is rounded to a whole number, which then stands for the reference everywhere: d_j is one fused multiply-add with no error but
+// its own, and a part seen from another reference is multiplied by a power of two, exactly.  (The hardware's exponential is 3.4e-9 too small on average, and an element would go
 // through four of them on its way into S.)
 //
 // Where |m c| reaches 2^24 ("low" rows: nothing but a mask's value, -1e9 or the lowest of the type) the next whole number can be
@@ -118,7 +119,7 @@ struct Part {
   float m, s, w;
 };
 
-constexpr float LOW = 0x1p24f, FAR = 0x1p80f;
+constexpr float LOW = 0x1p24f;
 
 // A reference and its product with c as a whole number.
 struct Ref {
@@ -512,48 +513,44 @@ struct Row : Span<T, TPR> {
   template <bool WANT_W, typename F>
   __device__ __forceinline__ Part stats(float c, const F& leave_out) {
     const float beside = leave_out.extra(t, extra());
-    float g = beside;
-    if (slots > 0) {
-      float f[VEC];
-      elements(0, f);
-      leave_out.vector(0, t, f);
+    Part p{-INFINITY, 0.f, 0.f};                                // an empty part, which no other one is seen from
+    Ref ref = make_ref(-INFINITY, c);
+    float limit = -INFINITY;
+    const float bit = __builtin_amdgcn_rcpf(c);
+    // One reference for the wave, in a scalar register, and another where any lane has an element more than a bit above it; what
+    // was added up before is multiplied by a power of two.
+    const auto raise = [&](float g, float& s, float& w) {
+      if (!__any(g > limit)) return;
+      const float m = lanes_max(g);
+      ref = make_ref(m, c);
+      rebase(p.s, p.w, p.m, ref, c);
+      rebase(s, w, p.m, ref, c);
+      p.m = m;
+      limit = m + bit;
+    };
+    float none = 0.f, none_w = 0.f;
+    raise(beside, none, none_w);
+    if (!ref.low) add_up<1, false, WANT_W>(&beside, ref, c, p.s, p.w);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) g = fmaxf(g, f[j]);
-    }
-    g = lanes_max(g);                                           // one reference for the wave, in a scalar register
-    if (g == -INFINITY) {                                       // nothing there (a mask): all that the wave holds
+    for (int i = 0; i < NCH; i += 4) {
+      float s = 0.f, w = 0.f;
 #pragma unroll
-      for (int i = 1; i < NCH; ++i)
-        if (i < slots) {
+      for (int k = 0; k < 4; ++k)
+        if (i + k < slots && !ref.low) {
           float f[VEC];
-          elements(i, f);
-          leave_out.vector(i, t, f);
+          elements(i + k, f);
+          leave_out.vector(i + k, t, f);
+          float g = f[0];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) g = fmaxf(g, f[j]);
+          for (int j = 1; j < VEC; ++j) g = fmaxf(g, f[j]);
+          raise(g, s, w);
+          if (!ref.low) add_up<VEC, false, WANT_W>(f, ref, c, s, w);
         }
-      g = lanes_max(g);
-    }
-    const Ref ref = make_ref(g, c);
-    Part p{g, 0.f, 0.f};                                        // -inf still: an empty part, which no other one is seen from
-    if (!ref.low) {
-      add_up<1, false, WANT_W>(&beside, ref, c, p.s, p.w);
-#pragma unroll
-      for (int i = 0; i < NCH; i += 4) {
-        float s = 0.f, w = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (i + k < slots) {
-            float f[VEC];
-            elements(i + k, f);
-            leave_out.vector(i + k, t, f);
-            add_up<VEC, false, WANT_W>(f, ref, c, s, w);
-          }
-        p.s += s;
-        p.w += w;
-      }
+      p.s += s;
+      p.w += w;
     }
     int from = NCH;
-    if (ref.low || !__all(p.s < FAR)) {                         // another reference is needed: again, with the largest so far
+    if (ref.low) {                                              // element by element, from the beginning
       p = Part{-INFINITY, 0.f, 0.f};
       take<1, WANT_W>(p, &beside, c);
       from = 0;

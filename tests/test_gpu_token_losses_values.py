@@ -164,3 +164,50 @@ def test_distill_a_position_without_entries_contributes_nothing(vocab, tail):
     assert not leaf.grad[:4].any() and leaf.grad[4].any()
     (2 * topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)).backward()      # computed again
     assert not leaf.grad[:4].any()
+
+
+# ---- rows with one dominant logit ---------------------------------------------------------------------------------------------------
+#: a row for each kernel: a wave's and a block's, held and in part read again
+ROWS = [(torch.float32, 1000), (torch.bfloat16, 2040), (torch.float16, 7001), (torch.bfloat16, 16000), (torch.float32, 16001),
+        (torch.bfloat16, 50001), (torch.bfloat16, 80000), (torch.bfloat16, 131072), (torch.float32, 131072)]
+
+
+@pytest.mark.parametrize("dtype,vocab", ROWS)
+@pytest.mark.parametrize("gap", [30.0, 38.0, 45.0, 52.0])
+def test_policy_of_a_token_that_the_model_is_sure_of(dtype, vocab, gap):
+    """The dominant logit is far above the first vectors of its row, and of its wave; the model's log-probability is its own old
+    one.  All others together are below V exp(0.5 - gap) <= 2e-8 of the sum, so that adding them in any order changes it by no more
+    than that: what is left is the dominant element's own error, 2 U of the exponential and U of its argument, which therefore
+    has to be near 0."""
+    from style_transfer_amd.losses import clipped_policy_loss, token_logprobs
+    n = 3
+    x = torch.randn(n, vocab, generator=torch.Generator().manual_seed(vocab))
+    at = torch.tensor([vocab * 3 // 5, vocab - 1, vocab // 2 + 1])
+    x[torch.arange(n), at] = gap
+    x = x.to(dtype)
+    label = at.clone()
+    label[2] = 0                                                # an improbable token, and a ratio of 1 as well
+    logp, h, log_q, q = O.token_logprobs(x, label)
+    old = logp.float()
+    others = vocab * math.exp(1.0 - gap)
+    err = others + 4 * U
+    for r in range(n):
+        leaf = x[r:r + 1].cuda().requires_grad_(True)
+        got = clipped_policy_loss(leaf[None], label[r:r + 1][None].cuda(), old[r:r + 1][None].cuda(), torch.ones(1, 1).cuda(), entropy_coef=0.01)
+        got.loss.backward()
+        ratio = math.exp(float(logp[r]) - float(old[r]))
+        stats = got.stats.cpu().double()
+        assert abs(float(stats[0]) + ratio) <= ratio * (err + U)
+        # H = ln S - ln2 W / S: the argument's share of the dominant element, at most 2 bits, cancels but for three roundings
+        assert abs(float(stats[2]) - float(h[r])) <= err + gap * others + 2 * math.log(2) * 3 * U
+        a = torch.tensor([-ratio], dtype=torch.float64)
+        _, _, want = O.policy(x[r:r + 1], label[r:r + 1], [(0, 1)], old[r:r + 1], torch.ones(1), ent=0.01)
+        grad = leaf.grad.cpu().double()
+        half = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+        tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+        bound = a.abs() * q[r] * (err + 6 * U + (log_q[r] - log_q[r].max()).abs().clamp(max=200) * 2 * U) + want.abs() * half * 1.01 + tiny
+        bound[0, label[r]] += 4 * U                             # 1 - q there
+        bound += 0.01 * q[r] * (log_q[r].abs().clamp(max=200) + h[r]) * (err + 40 * U)
+        assert bool(((grad - want).abs() <= bound).all())
+    both = clipped_policy_loss(x[None].cuda(), label[None].cuda(), token_logprobs(x.cuda(), label.cuda())[None], torch.ones(1, n).cuda())
+    assert abs(float(both.stats[0]) + 1) <= 2 * err + float(logp.abs().max()) * U        # an old log-probability is rounded to fp32
