@@ -305,7 +305,7 @@ __device__ __forceinline__ TokenTerms token_terms(double log_ratio, double d, co
   t.kl = 0;
   if (q.ref) {
     t.kl = kl_estimate(d);
-    if (q.kl != 0) t.a -= q.kl * (t.kl + d);
+    if (q.kl != 0) t.a -= q.kl * (d == -INFINITY ? -1.0 : t.kl + d);     // exp(d) - 1
   }
   return t;
 }

@@ -211,3 +211,24 @@ def test_policy_of_a_token_that_the_model_is_sure_of(dtype, vocab, gap):
         assert bool(((grad - want).abs() <= bound).all())
     both = clipped_policy_loss(x[None].cuda(), label[None].cuda(), token_logprobs(x.cuda(), label.cuda())[None], torch.ones(1, n).cuda())
     assert abs(float(both.stats[0]) + 1) <= 2 * err + float(logp.abs().max()) * U        # an old log-probability is rounded to fp32
+
+
+# ---- policy: a token that another model rules out -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("vocab", [50, 9000])
+def test_policy_reference_that_masks_the_token(vocab):
+    """ref = -inf: the estimate is +inf, its derivative -kl_coef (exp(ref - logp) - 1) = kl_coef."""
+    from style_transfer_amd.losses import clipped_policy_loss
+    x = torch.randn(2, vocab, generator=torch.Generator().manual_seed(9))
+    t = torch.tensor([3, 4])
+    logp, h, log_q, q = O.token_logprobs(x, t)
+    ref = torch.stack([torch.tensor(-INF), logp[1].float() - 0.5])
+    leaf = x.cuda().requires_grad_(True)
+    got = clipped_policy_loss(leaf[None], t[None].cuda(), logp.float()[None].cuda(), torch.zeros(1, 2).cuda(), ref[None].cuda(), kl_coef=0.25)
+    got.loss.backward()
+    assert float(got.loss.detach()) == INF and float(got.stats[1]) == INF
+    a = torch.stack([torch.tensor(0.125, dtype=torch.float64), -0.125 * torch.expm1(ref[1].double() - logp[1])])
+    want = O.row_gradient(t, 1.0, h, log_q, q, a, a * 0)
+    err = (vocab / 64 + 64) * U                                # a row's; an entry of it has 40 bits of its exponent besides
+    bound = a.abs()[:, None] * q * (2 * err + 80 * U) + want.abs() * 4 * U + 0.125 * 2 * err * (q > 0.01)
+    bound[torch.arange(2), t] += 0.125 * (2 * err + 8 * U)
+    assert bool(((leaf.grad.cpu().double() - want).abs() <= bound + 2.0 ** -126).all())
