@@ -262,7 +262,7 @@ __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, 
 }
 
 __device__ __forceinline__ void no_list(const ListIn& q, const Sums& u, unsigned r, int t) {
-  if (t == 0) u.terms[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (t == 0) u.terms[r] = f64x4{0.0, 0.0, 0.0, 0.0};
   if (t < 2 && q.row) q.row[2 * (size_t)r + t] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
@@ -332,9 +332,9 @@ __global__ __launch_bounds__(S::BLOCK, 4) void distill_kernel(Logits p, ListIn q
     if (TPR > 64) list = join_lists(p, q, threadIdx.x < TPR / 64 ? lists[threadIdx.x] : ListSum{0.0, 0.0, -INFINITY, 0.f, -INFINITY, 0, 0});
     if (twice) list = without_repeats(p, q, r, x, list);
     const double w = q.mask ? one_over(share) : 1.0 / u.rows;
-    const float loss = (float)(w * p.tau * p.tau * finish_list(p, q, m, list, w, twice, a, b));
+    const double loss = w * p.tau * p.tau * finish_list(p, q, m, list, w, twice, a, b);
     if (t == 0) {
-      u.terms[r] = f32x4{loss, 0.f, 0.f, 0.f};
+      u.terms[r] = f64x4{loss, 0.0, 0.0, 0.0};
       if (q.row) {
         q.row[2 * (size_t)r] = a;
         q.row[2 * (size_t)r + 1] = b;

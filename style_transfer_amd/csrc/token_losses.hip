@@ -32,7 +32,7 @@ struct StatsOut {
 // (m, 1 / (tau S), H - ln S, -).
 template <typename T>
 __device__ __forceinline__ void write_row(const Logits& p, unsigned r, long long label, const Part& q, const StatsOut& o) {
-  const RowStat st = finish<true>(q, p);
+  const RowStat st = finish(q, p);
   double lp = NAN;
   float inv = st.inv_ts;
   if (label >= 0 && label < p.vocab) lp = log_prob(load_one<T>(p.x, row_offset(p, r) + label), st, p);
@@ -281,23 +281,21 @@ struct TokenTerms {
   double a;                  // d (surrogate + kl_coef KL) / d logp
 };
 
-// exp(d) - 1 - d, which is all that is left of it near 0: its series up to |d| = 1
+// exp(d) - 1 - d, which is all that is left of it near 0: its series up to |d| = 1/4 (the term left out is below 2^-36 of it)
 __device__ __forceinline__ double kl_estimate(double d) {
-  if (!(fabs(d) <= 1.0)) {
-    const double e = (double)exp_wide(d);
+  if (!(fabs(d) <= 0.25)) {
+    const double e = exp64(d);
     return e == INFINITY ? e : e - 1.0 - d;
   }
-  const float v = (float)d;
-  float s = 1.f / 39916800.f;                                   // sum of d^n / n! from n = 2; the term left out is below 2^-27 of it
-  constexpr float f[] = {1.f / 3628800.f, 1.f / 362880.f, 1.f / 40320.f, 1.f / 5040.f, 1.f / 720.f, 1.f / 120.f, 1.f / 24.f, 1.f / 6.f, 0.5f};
+  double s = 1.0;
 #pragma unroll
-  for (int n = 0; n < 9; ++n) s = fmaf(s, v, f[n]);
-  return (double)(s * v) * d;
+  for (int n = 9; n > 2; --n) s = fma(s * d, 1.0 / n, 1.0);
+  return 0.5 * d * d * s;
 }
 
 __device__ __forceinline__ TokenTerms token_terms(double log_ratio, double d, const PolicyIn& q, double adv) {
   TokenTerms t;
-  const double ratio = (double)exp_wide(log_ratio);
+  const double ratio = exp64(log_ratio);
   const bool over = adv > 0 && ratio > 1 + q.high, under = adv < 0 && ratio < 1 - q.low;
   t.clipped = over || under;
   t.part = -adv * (over ? 1 + q.high : under ? 1 - q.low : ratio);
@@ -373,7 +371,7 @@ __global__ __launch_bounds__(S::BLOCK, 4) void policy_kernel(Logits p, PolicyIn 
   T* out = grad ? grad + (size_t)r * p.vocab : nullptr;
   if (label == p.ignore || s < 0) {
     if (t == 0) {
-      u.terms[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+      u.terms[r] = f64x4{0.0, 0.0, 0.0, 0.0};
       if (q.row) q.row[r] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     if (out) store_zeros<T, TPR>(out, p.vocab, t);
@@ -393,7 +391,7 @@ __global__ __launch_bounds__(S::BLOCK, 4) void policy_kernel(Logits p, PolicyIn 
   f32x4 g{0.f, 0.f, 0.f, 0.f};
   if (TPR == 64 || threadIdx.x < 64) {
     const double w = one_over(share) / own;
-    const RowStat st = finish<false>(m, p);
+    const RowStat st = finish(m, p);
     const double logp = inside ? log_prob((float)x_label, st, p) : NAN;
     const TokenTerms k = token_terms(logp - (double)old, (double)ref - logp, q, (double)adv);
     if (st.inv_ts != 0.f) {
@@ -401,7 +399,7 @@ __global__ __launch_bounds__(S::BLOCK, 4) void policy_kernel(Logits p, PolicyIn 
       g = f32x4{st.ref, (float)(-(a + b * ((double)st.h - st.ln_s)) * over), (float)(-b * p.inv_ct * over), (float)(a * p.inv_tau)};
     }
     if (t == 0) {
-      u.terms[r] = f32x4{(float)(w * k.part), (float)(w * k.kl), (float)(w * (double)st.h), (float)(w * k.clipped)};
+      u.terms[r] = f64x4{w * k.part, w * k.kl, w * (double)st.h, w * k.clipped};
       if (q.row) q.row[r] = g;
       if (TPR > 64) told = g;
     }

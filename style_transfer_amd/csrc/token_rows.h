@@ -37,6 +37,7 @@ constexpr float D_MIN = -200.f;          // 2^-200 is 0 in fp32: keeps 0 * inf o
 constexpr double LN2 = 0.6931471805599453094;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_u __attribute__((aligned(2)));      // a row of another alignment than the one loaded
 
@@ -283,13 +284,6 @@ __device__ __forceinline__ double ln_wide(float v) {
   return (double)(__builtin_amdgcn_frexp_expf(v) - up) * LN2 + (double)(__builtin_amdgcn_logf(up ? 2 * f : f) * (float)LN2);
 }
 
-// exp(v), relative error of about 2^-23 whatever the size of v
-__device__ __forceinline__ float exp_wide(double v) {
-  if (v != v) return (float)v;
-  const double y = fmax(fmin(v * (1.0 / LN2), 1000.0), -1000.0), k = rint(y);      // 2^1000 and 2^-1000 are inf and 0 here
-  return ldexpf(__builtin_amdgcn_exp2f((float)(y - k)), (int)k);
-}
-
 // exp(v), relative error below 2^-46: the 16th root's series (the term left out is below 2^-47 of the result), squared four times with
 // 1 left out.  (The library's exp is exact to the last bit and takes 24 registers more of kernels that hold a row in theirs.)
 __device__ __forceinline__ double exp64(double v) {
@@ -303,6 +297,12 @@ __device__ __forceinline__ double exp64(double v) {
   return ldexp(1.0 + p, (int)k);
 }
 
+// ln v, absolute error below 2^-46: what exp64 leaves of the logarithm above, to second order (of 1e-7)
+__device__ __forceinline__ double ln64(double v) {
+  const double y = ln_wide((float)v), left = fma(v, exp64(-y), -1.0);
+  return fma(-0.5 * left, left, left) + y;
+}
+
 __device__ __forceinline__ float reciprocal(float v) {
   const float r = __builtin_amdgcn_rcpf(v);
   return fmaf(fmaf(-v, r, 1.f), r, r);
@@ -311,16 +311,13 @@ __device__ __forceinline__ float reciprocal(float v) {
 // what a reference is in x / tau
 __device__ __forceinline__ double logit_of(const Ref& r, const Logits& p) { return r.low ? (double)r.m * p.inv_tau : (double)r.mc * p.inv_ct; }
 
-// SUMMED: log-probabilities that a caller adds up over hundreds of tokens, where a mean error counts: ln_wide's is 2e-8, the
-// fp64 logarithm leaves the exponential's 3.4e-9.
-template <bool SUMMED>
 __device__ __forceinline__ RowStat finish(const Part& q, const Logits& p) {
   RowStat r;
   const Ref ref = make_ref(q.m, p.c);
   const float inv = reciprocal(q.s);
   r.ref = ref.m;
   r.z = logit_of(ref, p);
-  r.ln_s = SUMMED ? log((double)q.s - (double)p.eps_ln2 * (double)q.w) : ln_wide(fmaf(-p.eps_ln2, q.w, q.s));
+  r.ln_s = ln64((double)q.s - (double)p.eps_ln2 * (double)q.w);
   r.h = (float)(r.ln_s - p.inv_ct * (double)q.w * (double)inv);
   r.inv_ts = (float)(p.inv_tau * (double)inv);
   if (q.s == 0.f) {
@@ -615,7 +612,7 @@ constexpr int COUNT_BLOCKS = 64;
 struct Sums {
   double* counted;           // [COUNT_BLOCKS]
   int blocks;                // of them used
-  f32x4* terms;              // [rows]: a row's weighted terms
+  f64x4* terms;              // [rows]: a row's weighted terms; of both signs, their sum may be far smaller than they are
   double* partial;           // [4][COUNT_BLOCKS]
   unsigned rows;
   float* loss;               // scale * (terms[0] + kl terms[1] - ent terms[2])
@@ -645,8 +642,8 @@ static __global__ __launch_bounds__(1024) void sum_terms_kernel(Sums q) {
   __shared__ double red[16];
   double sum[4] = {0, 0, 0, 0};
   for (unsigned r = blockIdx.x * 1024 + threadIdx.x; r < q.rows; r += gridDim.x * 1024) {
-    const f32x4 v = q.terms[r];
-    for (int k = 0; k < 4; ++k) sum[k] += (double)v[k];
+    const f64x4 v = q.terms[r];
+    for (int k = 0; k < 4; ++k) sum[k] += v[k];
   }
   for (int k = 0; k < 4; ++k) sum[k] = block_sum64(sum[k], red);
   if (threadIdx.x != 0) return;
@@ -717,7 +714,7 @@ inline Sums make_sums(Space& w, long long rows, float* loss, float* stats, doubl
   Sums q{};
   q.counted = w.take<double>(COUNT_BLOCKS);
   q.partial = w.take<double>(4 * COUNT_BLOCKS);
-  q.terms = w.take<f32x4>((size_t)rows);
+  q.terms = w.take<f64x4>((size_t)rows);
   q.rows = (unsigned)rows;
   q.loss = loss;
   q.stats = stats;
@@ -727,7 +724,7 @@ inline Sums make_sums(Space& w, long long rows, float* loss, float* stats, doubl
   return q;
 }
 
-inline size_t sums_bytes(long long rows) { return align256(COUNT_BLOCKS * 8) * 5 + align256((size_t)rows * sizeof(f32x4)); }
+inline size_t sums_bytes(long long rows) { return align256(COUNT_BLOCKS * 8) * 5 + align256((size_t)rows * sizeof(f64x4)); }
 
 inline void launch_sum_terms(const Sums& q, hipStream_t s) {
   const bool one = q.rows <= 16384;                             // 16 rows a thread

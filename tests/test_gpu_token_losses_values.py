@@ -232,3 +232,52 @@ def test_policy_reference_that_masks_the_token(vocab):
     bound = a.abs()[:, None] * q * (2 * err + 80 * U) + want.abs() * 4 * U + 0.125 * 2 * err * (q > 0.01)
     bound[torch.arange(2), t] += 0.125 * (2 * err + 8 * U)
     assert bool(((leaf.grad.cpu().double() - want).abs() <= bound + 2.0 ** -126).all())
+
+
+# ---- policy: a token's terms --------------------------------------------------------------------------------------------------------
+def one_token(old, adv=1.0, ref=None, vocab=8, **settings):
+    """stats and loss of one token over equal logits: S = V exactly, log-probability -ln V to the last digit of 64 bits."""
+    from style_transfer_amd.losses import clipped_policy_loss
+    x = torch.zeros(1, 1, vocab, device="cuda", requires_grad=True)
+    t = torch.zeros(1, 1, dtype=torch.long, device="cuda")
+    f = lambda v: None if v is None else torch.full((1, 1), v, device="cuda")  # noqa: E731
+    got = clipped_policy_loss(x, t, f(old), f(adv), f(ref), **settings)
+    got.loss.backward()
+    return got.stats.cpu().double(), float(got.loss.detach()), x.grad.cpu().double().view(-1)
+
+
+def test_policy_ratio_and_estimate_have_one_rounding():
+    """exp(logp - old) and exp(d) - 1 - d in 64 bits, rounded once."""
+    g = torch.Generator().manual_seed(1)
+    for vocab in (8, 4096):
+        logp = -math.log(vocab)
+        for old, ref in zip((logp + torch.randn(24, generator=g)).tolist(), (logp + torch.randn(24, generator=g) * 2).tolist()):
+            old, ref = float(torch.tensor(old)), float(torch.tensor(ref))
+            stats, loss, _ = one_token(old, -1.0, ref, vocab, clip_high=1e30, clip_low=0.0)      # A < 0: the ratio above 1 is not held
+            ratio, d = max(1.0, math.exp(logp - old)), ref - logp
+            assert abs(float(stats[0]) - ratio) <= 1.001 * U * ratio
+            kl = math.expm1(d) - d
+            assert abs(float(stats[1]) - kl) <= 1.001 * U * kl
+
+
+def test_policy_advantage_of_zero_costs_nothing():
+    """0 times a ratio that fp32 cannot hold, but 64 bits can."""
+    stats, loss, grad = one_token(-120.0, adv=0.0)
+    assert loss == 0 and not stats[0] and not grad.any()
+
+
+def test_policy_terms_that_cancel():
+    """Rows' terms of both signs, whose sum is far smaller than they are: rounded once, at the end."""
+    from style_transfer_amd.losses import clipped_policy_loss
+    n, vocab = 200, 8
+    g = torch.Generator().manual_seed(5)
+    old = (-math.log(vocab) + torch.randn(n, generator=g) * 0.05)
+    adv = torch.randn(n, generator=g) * 1000
+    terms = -adv.double() * torch.exp(-math.log(vocab) - old.double())
+    adv[-1] += float(terms.sum() / torch.exp(-math.log(vocab) - old.double())[-1])
+    terms = -adv.double() * torch.exp(-math.log(vocab) - old.double())
+    want = float(terms.mean())
+    assert abs(want) < 1e-4 * float(terms.abs().mean())
+    x, t = torch.zeros(n, 1, vocab, device="cuda"), torch.zeros(n, 1, dtype=torch.long, device="cuda")
+    got = clipped_policy_loss(x, t, old[:, None].cuda(), adv[:, None].cuda(), clip_low=0.9, clip_high=9.0)
+    assert abs(float(got.loss) - want) <= 1.001 * U * abs(want) + float(terms.abs().mean()) * 2.0 ** -48
