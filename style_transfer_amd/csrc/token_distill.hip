@@ -25,7 +25,7 @@ constexpr size_t MAX_PLAIN_LDS = 48 << 10;   // dynamic LDS that a kernel gets w
 struct ListSum {
   double z;                  // sum of exp((v - vref) / tau); tail: the mass itself
   double gap;                // sum of exp((v - vref) / tau) ((v - vref) / tau - (x - m) / tau)
-  float m, s;                // the listed logits' maximum, S of the listed tokens seen from it (once each entry)
+  float m, s, w;             // the listed logits' maximum, S and W of the listed tokens seen from it (once each entry)
   float vref;                // the values' maximum, -inf without any; tail: 0
   int used, bad;             // entries; any outside the vocabulary
 };
@@ -88,7 +88,7 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
   o.bad = __any(bad);
   const Ref ref = make_ref(o.m, p.c);
   const double it = q.tail ? 1.0 : p.inv_tau, from = o.vref == -INFINITY ? 0.0 : (double)o.vref;
-  float s = 0.f;
+  float s = 0.f, w = 0.f;
   double z = 0.0, gap = 0.0;
   e = mine;
   for (int i = k;;) {
@@ -96,6 +96,7 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
       const float d = distance((float)e.x, ref, p.c), ex = __builtin_amdgcn_exp2f(d);
       const double lv = ((double)e.v - from) * it, ev = exp64(lv);      // 64 bits: 1 - sum p has no digit left of a p rounded to 32
       s += ex;
+      w = fmaf(fmaxf(d, D_MIN), ex, w);
       z += ev;
       if (ev != 0.0) gap += ev * (lv - ((double)(float)e.x - (double)ref.m) * p.inv_tau);
     }
@@ -103,6 +104,7 @@ __device__ __forceinline__ ListSum sum_list(const Logits& p, const ListIn& q, un
     e = load_entry(p, q, r, i, x);
   }
   o.s = lanes_sum(s);
+  o.w = lanes_sum(w);
   o.z = lanes_sum(z);
   o.gap = lanes_sum(gap);
   return o;
@@ -114,14 +116,15 @@ __device__ __forceinline__ ListSum join_lists(const Logits& p, const ListIn& q, 
   o.m = lanes_max<16>(part.m);
   o.vref = q.tail ? 0.f : lanes_max<16>(part.vref);
   const Ref ref = make_ref(o.m, p.c);
-  float s = part.s, unused = 0.f;
-  rebase(s, unused, part.m, ref, p.c);
+  float s = part.s, w = part.w;
+  rebase(s, w, part.m, ref, p.c);
   // (v - vref) / tau and (x - m) / tau of the part's entries change by a and b
   const bool any = part.z != 0;
   const double a = !any || q.tail ? 0.0 : ((double)part.vref - (double)o.vref) * p.inv_tau;
   const double b = any && part.m > -INFINITY ? ((double)part.m - (double)ref.m) * p.inv_tau : 0.0;
   const double f = any ? exp64(a) : 0.0;
   o.s = lanes_sum<16>(s);
+  o.w = lanes_sum<16>(w);
   o.z = lanes_sum(any ? f * part.z : 0.0);
   o.gap = lanes_sum(f != 0.0 ? f * (part.gap + part.z * (a - b)) : 0.0);      // an entry without mass does not count: its logit may be -inf
   o.used = (int)lanes_sum<16>((float)part.used);
@@ -208,16 +211,21 @@ template <typename T>
 __device__ __forceinline__ ListSum without_repeats(const Logits& p, const ListIn& q, unsigned r, const T* x, ListSum o) {
   const size_t first = (size_t)r * q.k;
   const Ref ref = make_ref(o.m, p.c);
-  float s = 0, n = 0;
+  float s = 0, w = 0, n = 0;
   for (int k = threadIdx.x & 63; k < q.k; k += 64) {
     const int j = entry_index(q, first + k, p.vocab);
     bool again = false;
     if (j >= 0)
       for (int i = 0; i < k; ++i) again |= entry_index(q, first + i, p.vocab) == j;      // no exit: the loads overlap
     if (again) n += 1;
-    else if (j >= 0) s += __builtin_amdgcn_exp2f(distance((float)x[j], ref, p.c));
+    else if (j >= 0) {
+      const float d = distance((float)x[j], ref, p.c), ex = __builtin_amdgcn_exp2f(d);
+      s += ex;
+      w = fmaf(fmaxf(d, D_MIN), ex, w);
+    }
   }
   o.s = lanes_sum(s);
+  o.w = lanes_sum(w);
   o.used -= (int)lanes_sum(n);
   return o;
 }
@@ -227,23 +235,22 @@ __device__ __forceinline__ double finish_list(const Logits& p, const ListIn& q, 
                                               f32x4& a, f32x4& b) {
 #pragma clang fp contract(off)                                  // two equal references over tau have no difference
   const Ref ref = make_ref(fmaxf(off.m, o.m), p.c), ref_off = make_ref(off.m, p.c);
-  // W is not kept here (it costs a sixth of the pass over the row): what it would take out of ln S, c's rounding times the mean
-  // distance from the reference, is below 1e-7, and these rows are not summed against another model's
-  float s_off = off.s, s_list = o.s, unused = 0.f;
-  rebase(s_off, unused, off.m, ref, p.c);
-  rebase(s_list, unused, o.m, ref, p.c);
+  float s_off = off.s, w_off = off.w, s_list = o.s, w_list = o.w;
+  rebase(s_off, w_off, off.m, ref, p.c);
+  rebase(s_list, w_list, o.m, ref, p.c);
   const float s = s_list + s_off;
-  const double from = logit_of(ref, p), ln_s = ln_wide(s);      // their sum is ln of the sum of exp(x / tau); references are
-                                                                // subtracted from each other first: they may be -1e14
+  const double eps = (double)p.eps_ln2;                         // takes c's rounding out of ln S
+  const double from = logit_of(ref, p), ln_s = ln64((double)s - eps * (double)(w_list + w_off));      // their sum is ln of the sum of
+                                                                // exp(x / tau); references are subtracted from each other first: they may be -1e14
   const double mass = q.tail ? o.z : o.z == 0 ? 0.0 : o.z / o.z;                       // 1, or NaN
   double loss = 0;
   if (mass != 0) {
-    loss = (q.tail ? o.gap : o.gap / o.z - ln_wide((float)o.z)) + mass * (from - (double)make_ref(o.m, p.c).m * p.inv_tau + ln_s);
+    loss = (q.tail ? o.gap : o.gap / o.z - ln64(o.z)) + mass * (from - (double)make_ref(o.m, p.c).m * p.inv_tau + ln_s);
     if (s == 0.f) loss = INFINITY;
   }
   const double rest = q.tail && o.used < p.vocab ? (mass < 1 ? 1 - mass : mass >= 1 ? 0.0 : mass) : 0.0;
   const float inv = reciprocal(s), inv_off = reciprocal(off.s);
-  if (rest != 0) loss += off.s == 0.f ? INFINITY : rest * (ln_wide((float)rest) - (logit_of(ref_off, p) - from + (ln_wide(off.s) - ln_s)));
+  if (rest != 0) loss += off.s == 0.f ? INFINITY : rest * (ln64(rest) - (logit_of(ref_off, p) - from + (ln64((double)off.s - eps * (double)off.w) - ln_s)));
   const double gr = q.scale * weight * p.tau, total = mass + rest;
   const float on = s == 0.f ? 0.f : (float)(gr * total * (double)inv);
   const double back = (double)__builtin_amdgcn_exp2f(step(off.m, ref, p.c));
@@ -323,13 +330,13 @@ __global__ __launch_bounds__(S::BLOCK, 4) void distill_kernel(Logits p, ListIn q
   row.load();
   const double share = q.mask ? counted_share(u) : 0.0;
   twice = sync_row_or<TPR>(twice);
-  ListSum list{0.0, 0.0, -INFINITY, 0.f, -INFINITY, 0, 0};
+  ListSum list{0.0, 0.0, -INFINITY, 0.f, 0.f, -INFINITY, 0, 0};
   if (has_entries) list = sum_list(p, q, r, x, mine, t, TPR);
   if (TPR > 64 && (threadIdx.x & 63) == 0) lists[threadIdx.x >> 6] = list;     // read behind row_join's barrier
-  const Part m = row_join<TPR>(row.template stats<false>(p.c, Unlisted<M>{marks, words - 1}), p.c, red);
+  const Part m = row_join<TPR>(row.stats(p.c, Unlisted<M>{marks, words - 1}), p.c, red);
   f32x4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
   if (TPR == 64 || threadIdx.x < 64) {
-    if (TPR > 64) list = join_lists(p, q, threadIdx.x < TPR / 64 ? lists[threadIdx.x] : ListSum{0.0, 0.0, -INFINITY, 0.f, -INFINITY, 0, 0});
+    if (TPR > 64) list = join_lists(p, q, threadIdx.x < TPR / 64 ? lists[threadIdx.x] : ListSum{0.0, 0.0, -INFINITY, 0.f, 0.f, -INFINITY, 0, 0});
     if (twice) list = without_repeats(p, q, r, x, list);
     const double w = q.mask ? one_over(share) : 1.0 / u.rows;
     const double loss = w * p.tau * p.tau * finish_list(p, q, m, list, w, twice, a, b);

@@ -387,7 +387,7 @@ __global__ __launch_bounds__(S::BLOCK, 4) void policy_kernel(Logits p, PolicyIn 
   const float old = q.old_logp[r], ref = q.ref ? q.ref[r] : 0.f, adv = q.adv[q.adv_per_sequence ? s : r];
   const double share = counted_share(u);
   const int own = q.per_sequence ? q.count[s] : 1;
-  const Part m = row_join<TPR>(row.template stats<true>(p.c, Whole{}), p.c, red);
+  const Part m = row_join<TPR>(row.stats(p.c, Whole{}), p.c, red);
   f32x4 g{0.f, 0.f, 0.f, 0.f};
   if (TPR == 64 || threadIdx.x < 64) {
     const double w = one_over(share) / own;

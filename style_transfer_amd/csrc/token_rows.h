@@ -229,8 +229,7 @@ __device__ __forceinline__ Part row_join(Part p, float c, Part* red) {
 // e_j and e_j d_j of N elements, each group of four summed by itself first: where one element is most of S, what it is
 // added to loses the small ones' last digits all in one direction, and a row of 131072 has hundreds of them a thread
 // (measured on rows with one such element: ln S 1.3e-6 too small on average with one running sum).
-// WANT_W: W as well.
-template <int N, bool IS_LOW, bool WANT_W>
+template <int N, bool IS_LOW>
 __device__ __forceinline__ void add_up(const float* x, const Ref& ref, float c, float& s, float& w) {
   float ss = 0.f, ww = 0.f;
 #pragma unroll
@@ -244,17 +243,15 @@ __device__ __forceinline__ void add_up(const float* x, const Ref& ref, float c, 
     }
     const float s4 = (e[0] + e[1]) + (e[2] + e[3]);
     ss = g == 0 ? s4 : ss + s4;
-    if (WANT_W) {
-      const float w4 = fmaf(a[1], e[1], a[0] * e[0]) + fmaf(a[3], e[3], a[2] * e[2]);
-      ww = g == 0 ? w4 : ww + w4;
-    }
+    const float w4 = fmaf(a[1], e[1], a[0] * e[0]) + fmaf(a[3], e[3], a[2] * e[2]);
+    ww = g == 0 ? w4 : ww + w4;
   }
   s += ss;
-  if (WANT_W) w += ww;
+  w += ww;
 }
 
 // N more elements into a thread's part, whose reference is the largest that it has seen
-template <int N, bool WANT_W = true>
+template <int N>
 __device__ __forceinline__ void take(Part& p, const float* x, float c) {
   float m = p.m;
 #pragma unroll
@@ -264,8 +261,8 @@ __device__ __forceinline__ void take(Part& p, const float* x, float c) {
     rebase(p.s, p.w, p.m, ref, c);
     p.m = m;
   }
-  if (ref.low) add_up<N, true, WANT_W>(x, ref, c, p.s, p.w);
-  else add_up<N, false, WANT_W>(x, ref, c, p.s, p.w);
+  if (ref.low) add_up<N, true>(x, ref, c, p.s, p.w);
+  else add_up<N, false>(x, ref, c, p.s, p.w);
 }
 
 // ---- what the logits of a row say once its parts are joined ----------------------------------------------------------------
@@ -507,7 +504,7 @@ struct Row : Span<T, TPR> {
 
   // The thread's part of the row's statistics.  `leave_out` puts -inf in place of what does not belong: among the elements f of
   // the thread's `slot`-th vector, and of the element outside the vectors.
-  template <bool WANT_W, typename F>
+  template <typename F>
   __device__ __forceinline__ Part stats(float c, const F& leave_out) {
     const float beside = leave_out.extra(t, extra());
     Part p{-INFINITY, 0.f, 0.f};                                // an empty part, which no other one is seen from
@@ -527,7 +524,7 @@ struct Row : Span<T, TPR> {
     };
     float none = 0.f, none_w = 0.f;
     raise(beside, none, none_w);
-    if (!ref.low) add_up<1, false, WANT_W>(&beside, ref, c, p.s, p.w);
+    if (!ref.low) add_up<1, false>(&beside, ref, c, p.s, p.w);
 #pragma unroll
     for (int i = 0; i < NCH; i += 4) {
       float s = 0.f, w = 0.f;
@@ -541,7 +538,7 @@ struct Row : Span<T, TPR> {
 #pragma unroll
           for (int j = 1; j < VEC; ++j) g = fmaxf(g, f[j]);
           raise(g, s, w);
-          if (!ref.low) add_up<VEC, false, WANT_W>(f, ref, c, s, w);
+          if (!ref.low) add_up<VEC, false>(f, ref, c, s, w);
         }
       p.s += s;
       p.w += w;
@@ -549,7 +546,7 @@ struct Row : Span<T, TPR> {
     int from = NCH;
     if (ref.low) {                                              // element by element, from the beginning
       p = Part{-INFINITY, 0.f, 0.f};
-      take<1, WANT_W>(p, &beside, c);
+      take<1>(p, &beside, c);
       from = 0;
     }
     for (int slot = from; t + slot * TPR < nv; slot += AGAIN) {
@@ -567,7 +564,7 @@ struct Row : Span<T, TPR> {
           for (int j = 0; j < VEC; ++j) f[k * VEC + j] = -INFINITY;
         }
       }
-      take<AGAIN * VEC, WANT_W>(p, f, c);
+      take<AGAIN * VEC>(p, f, c);
     }
     return p;
   }

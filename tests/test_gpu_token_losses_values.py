@@ -281,3 +281,24 @@ def test_policy_terms_that_cancel():
     x, t = torch.zeros(n, 1, vocab, device="cuda"), torch.zeros(n, 1, dtype=torch.long, device="cuda")
     got = clipped_policy_loss(x, t, old[:, None].cuda(), adv[:, None].cuda(), clip_low=0.9, clip_high=9.0)
     assert abs(float(got.loss) - want) <= 1.001 * U * abs(want) + float(terms.abs().mean()) * 2.0 ** -48
+
+
+# ---- distillation: the rounding of log2(e) / tau --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1000), (torch.float32, 16384), (torch.bfloat16, 32768)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_at_a_temperature_that_rounds_badly(dtype, vocab, tail):
+    """tau for which log2(e) / tau lies between two fp32 numbers, 5.8e-8 of it away from either, and rows half of whose mass is far
+    below the other half: every ln S would be off in the same direction by that times the mean distance, about 5 U.  Over 64 rows
+    what is random goes down: a row's sum has up to 10 joins of U each, 10 U / sqrt(3 * 64) = 0.7 U of the mean, two of those are
+    1.4 U; the exponential's own mean error is 0.06 U."""
+    from style_transfer_amd.losses import topk_distill_loss
+    rows, tau = 64, 1 / (math.log(2) * (1 + 0.98 * 2.0 ** -24))
+    g = torch.Generator().manual_seed(vocab)
+    x = (torch.rand(rows, vocab, generator=g) - 0.5 - math.log(vocab)) * tau
+    x[torch.arange(rows), torch.arange(rows) * 3] = torch.rand(rows, generator=g) * 0.1
+    x = x.to(dtype)
+    idx = (torch.arange(rows) * 3)[:, None]
+    val = torch.full((rows, 1), math.log(0.5) if tail else 0.0)
+    loss, _ = O.distill(x, idx, val, None, tau, tail)
+    got = float(topk_distill_loss(x.cuda(), idx.cuda(), val.cuda(), temperature=tau, tail=tail))
+    assert abs(got - loss) <= tau * tau * 1.5 * U + U * abs(loss)
