@@ -19,7 +19,8 @@ What they have in common:
 * Results do not depend on the run: every sum has a fixed order.
 * ``clipped_policy_loss`` and ``topk_distill_loss`` write the gradient of logits that require one in the forward pass, while
   a row is on chip.  A backward pass with an upstream gradient of 1 hands it over; another one (a loss weight outside, a
-  dynamic loss scale) computes it again from the logits: pass a known factor as ``scale``.
+  dynamic loss scale) computes it again from the logits: pass a known factor as ``scale``.  Until then it is a saved tensor of
+  the logits' size beside them, and goes where saved tensors go.
 """
 from __future__ import annotations
 
@@ -239,19 +240,28 @@ def _wants_grad(x: torch.Tensor) -> bool:
 
 
 # ---- the two losses whose rows go through the label's log-probability -------------------------------------------------------------
-def _take_grad(ctx, x):
+def _keep(ctx, grad, *tensors):
+    """Saves what the backward pass reads, the gradient that the forward kernel wrote among it, so that saved-tensor hooks (the
+    host's memory, a checkpoint) reach it too.  ``data``: with a version of its own, since it is given away and may be changed."""
+    ctx.given = False
+    ctx.save_for_backward(*tensors, grad.data)
+
+
+def _take_grad(ctx, x, early):
     """(buffer, 1) the first time: it holds the gradient for an upstream gradient of 1, written by the forward kernel while the
     rows were on chip.  The buffer is given away, so a second backward pass gets a new one, (buffer, 0)."""
-    grad, ctx.grad = ctx.grad, None
-    return (_grad_buffer(x), 0) if grad is None else (grad, 1)
+    if ctx.given or not early:
+        return _grad_buffer(x), 0
+    ctx.given = True
+    return early[0].data, 1
 
 
 def _token_loss_bwd(ctx, gout):
     if gout is None:                                           # a node above has none for the loss
         return None, None
-    x, labels, row_grad = ctx.saved_tensors
+    x, labels, row_grad, *early = ctx.saved_tensors
     args, tau, ignore = ctx.call
-    grad, for_one = _take_grad(ctx, x)
+    grad, for_one = _take_grad(ctx, x, early)
     with _on(x):
         _lib.check(_lib.load().st_token_loss_bwd(*_place(x, args), *_label_args(labels, ignore), tau, row_grad.data_ptr(), gout.data_ptr(), for_one,
                                                  grad.data_ptr(), _lib.stream_ptr()), "st_token_loss_bwd")
@@ -277,7 +287,7 @@ class _PreferenceFunction(torch.autograd.Function):
         loss, rewards, buffer = _preference_fwd(x, call, True)
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
-        ctx.call, ctx.grad = (call[0], 1.0, call[2]), None
+        ctx.call, ctx.given = (call[0], 1.0, call[2]), False
         ctx.save_for_backward(x, call[1], buffer)
         return loss, rewards
 
@@ -345,11 +355,11 @@ def _policy_fwd(x, call, need):
 class _PolicyFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        loss, stats, ctx.grad, buffer = _policy_fwd(x, call, True)
+        loss, stats, grad, buffer = _policy_fwd(x, call, True)
         ctx.mark_non_differentiable(stats)
         ctx.set_materialize_grads(False)
         ctx.call = call[0], call[3], call[2]
-        ctx.save_for_backward(x, call[1], buffer)
+        _keep(ctx, grad, x, call[1], buffer)
         return loss, stats
 
     @_backward
@@ -413,16 +423,16 @@ def _distill_fwd(x, call, need):
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        loss, ctx.grad, buffer = _distill_fwd(x, call, True)
+        loss, grad, buffer = _distill_fwd(x, call, True)
         ctx.call = call[0], call[4], call[5]
-        ctx.save_for_backward(x, call[1], call[2], buffer)
+        _keep(ctx, grad, x, call[1], call[2], buffer)
         return loss
 
     @_backward
     def backward(ctx, gout):
-        x, idx, val, row_grad = ctx.saved_tensors
+        x, idx, val, row_grad, *early = ctx.saved_tensors
         args, tau, tail = ctx.call
-        grad, for_one = _take_grad(ctx, x)
+        grad, for_one = _take_grad(ctx, x, early)
         with _on(x):
             _lib.check(_lib.load().st_distill_loss_bwd(*_place(x, args), idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1], tau, tail,
                                                        row_grad.data_ptr(), gout.data_ptr(), for_one, grad.data_ptr(), _lib.stream_ptr()),

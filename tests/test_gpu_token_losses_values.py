@@ -302,3 +302,61 @@ def test_distill_at_a_temperature_that_rounds_badly(dtype, vocab, tail):
     loss, _ = O.distill(x, idx, val, None, tau, tail)
     got = float(topk_distill_loss(x.cuda(), idx.cuda(), val.cuda(), temperature=tau, tail=tail))
     assert abs(got - loss) <= tau * tau * 1.5 * U + U * abs(loss)
+
+
+# ---- the gradient that the forward pass leaves --------------------------------------------------------------------------------------
+def early(t, idx, val, old):
+    from style_transfer_amd import losses
+    return [lambda v: losses.clipped_policy_loss(v, t, old, old + 9).loss, lambda v: losses.topk_distill_loss(v, idx, val, tail=True)]
+
+
+def steps_of(vocab, seed=4):
+    from style_transfer_amd import losses
+    g = torch.Generator().manual_seed(seed)
+    x, t = torch.randn(4, 6, vocab, generator=g).cuda(), torch.randint(0, vocab, (4, 6), generator=g).cuda()
+    idx = torch.arange(24 * 5).view(4, 6, 5).cuda() % vocab
+    val = torch.log_softmax(torch.randn(4, 6, 5, generator=g), -1).cuda() - 0.1
+    return x, early(t, idx, val, losses.token_logprobs(x, t) + 0.1)
+
+
+def test_the_early_gradient_goes_where_saved_tensors_go():
+    """Saved tensors that are kept on the host, or dropped by a checkpoint: nothing of the logits' size stays on the device but the
+    logits themselves."""
+    from torch.utils.checkpoint import checkpoint
+    vocab = 60000
+    x, fns = steps_of(vocab)
+    size = x.numel() * 4
+    for fn in fns:
+        want = []
+        for mode in ("plain", "host", "checkpoint"):
+            leaf = x.clone().requires_grad_(True)
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            if mode == "host":
+                with torch.autograd.graph.save_on_cpu():
+                    loss = fn(leaf)
+            else:
+                loss = checkpoint(fn, leaf, use_reentrant=False) if mode == "checkpoint" else fn(leaf)
+            torch.cuda.synchronize()
+            held = torch.cuda.memory_allocated() - before
+            assert mode == "plain" or held < size // 4, (mode, held)
+            loss.backward()
+            want.append(leaf.grad)
+            del loss, leaf                                     # or the next measurement begins with them
+        assert torch.equal(want[0], want[1]) and torch.equal(want[0], want[2])
+
+
+def test_a_gradient_that_was_given_away_may_be_changed():
+    """Twice through one graph, with the first gradient changed in place between: the second is as the first was."""
+    x, fns = steps_of(700)
+    for fn in fns:
+        leaf = x.clone().requires_grad_(True)
+        loss = fn(leaf)
+        one, = torch.autograd.grad(loss, [leaf], retain_graph=True)
+        kept = one.clone()
+        one.mul_(7).add_(1)
+        two, = torch.autograd.grad(loss, [leaf], retain_graph=True)
+        assert torch.equal(two, kept)
+        two.zero_()
+        loss.backward()
+        assert torch.equal(leaf.grad, kept)
