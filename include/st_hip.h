@@ -54,6 +54,9 @@ typedef void* st_stream_t; /* hipStream_t */
 /* ---- library ------------------------------------------------------------------------ */
 int st_version(void);
 const char* st_last_error(void);
+/* Which capture of a graph a stream is in (the runtime's number of it), 0 outside of any: work that a graph will repeat may
+ * only rely on what the same graph repeats with it. */
+unsigned long long st_capture_id(st_stream_t stream);
 
 /* ---- 3x3 convolution (MFMA implicit GEMM) ---------------------------------------------
  * Replaces  SymmetricPadding2D((1,1,1,1)) -> nn.Conv2d(cin,cout,(3,3)) [-> nn.ReLU()]
@@ -524,7 +527,8 @@ int st_policy_loss_fwd(const void* x, int dtype, long long rows, long long inner
                        float* stats, float* row_grad, void* grad, void* workspace, st_stream_t stream);
 /* grad = gout[0] (NULL: 1) times the gradient of the preference or the policy loss, from their row_grad.
  * grad_is_for_one: grad holds the gradient for an upstream gradient of 1 already (st_policy_loss_fwd wrote it), and stays
- * as it is where gout[0] == 1. */
+ * as it is where gout[0] == 1.  In a graph only where the same graph holds that st_policy_loss_fwd: a replay finds in grad
+ * what the last one left. */
 int st_token_loss_bwd(const void* x, int dtype, long long rows, long long inner, long long s_outer,
                       long long s_inner, int vocab, const void* labels, int labels64, int ignore, double tau,
                       const float* row_grad, const float* gout, int grad_is_for_one, void* grad, st_stream_t stream);

@@ -22,6 +22,7 @@ _LABELS = [c_void_p, c_int, c_int]                                              
 SIGNATURES = {
     "st_version": (c_int, []),
     "st_last_error": (ctypes.c_char_p, []),
+    "st_capture_id": (ctypes.c_ulonglong, [c_void_p]),
     "st_conv3x3_packed_elems": (c_size_t, [c_int, c_int]),
     "st_conv3x3_pack_weights": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "st_conv3x3_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,

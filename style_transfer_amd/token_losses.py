@@ -243,14 +243,21 @@ def _wants_grad(x: torch.Tensor) -> bool:
 def _keep(ctx, grad, *tensors):
     """Saves what the backward pass reads, the gradient that the forward kernel wrote among it, so that saved-tensor hooks (the
     host's memory, a checkpoint) reach it too.  ``data``: with a version of its own, since it is given away and may be changed."""
-    ctx.given = False
+    ctx.given, ctx.capture = False, _capture(grad)
     ctx.save_for_backward(*tensors, grad.data)
+
+
+def _capture(x):
+    """The graph that is being captured, 0 outside of a capture."""
+    with _on(x):
+        return _lib.load().st_capture_id(_lib.stream_ptr())
 
 
 def _take_grad(ctx, x, early):
     """(buffer, 1) the first time: it holds the gradient for an upstream gradient of 1, written by the forward kernel while the
-    rows were on chip.  The buffer is given away, so a second backward pass gets a new one, (buffer, 0)."""
-    if ctx.given or not early:
+    rows were on chip.  The buffer is given away, so a second backward pass gets a new one, (buffer, 0); as does one that is
+    captured without its forward pass, since its replays would find in the buffer what the last of them left."""
+    if ctx.given or not early or ctx.capture != _capture(x):
         return _grad_buffer(x), 0
     ctx.given = True
     return early[0].data, 1

@@ -360,3 +360,62 @@ def test_a_gradient_that_was_given_away_may_be_changed():
         two.zero_()
         loss.backward()
         assert torch.equal(leaf.grad, kept)
+
+
+@pytest.mark.parametrize("vocab", [700, 20000])
+def test_a_backward_pass_in_a_graph_of_its_own(vocab):
+    """Forward and backward captured into two graphs, as make_graphed_callables does, and the second replayed more than once: each
+    replay gives the gradient for the upstream gradient that it finds, whatever the buffer held."""
+    x, fns = steps_of(vocab)
+    for fn in fns:
+        eager = x.clone().requires_grad_(True)
+        one, = torch.autograd.grad(fn(eager), [eager])
+        leaf, up = x.clone().requires_grad_(True), torch.ones((), device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(fn(leaf), [leaf], [up])
+        torch.cuda.current_stream().wait_stream(side)
+        forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(forward, stream=side):
+            loss = fn(leaf)
+        with torch.cuda.graph(backward, pool=forward.pool(), stream=side):
+            grad, = torch.autograd.grad(loss, [leaf], [up])
+        for first in range(3):
+            forward.replay()
+            for factor in (1.0, 3.0, 1.0, 0.0, 1.0):
+                up.fill_(factor)
+                backward.replay()
+                torch.cuda.synchronize()
+                assert torch.allclose(grad, one * factor, rtol=8 * U, atol=16 * U * 3 * float(one.abs().max())), factor
+                assert factor != 1 or torch.equal(grad, one)
+                grad.add_(0.25)                                 # the program's own use of it
+
+
+def test_the_early_gradient_is_used_where_its_forward_pass_is_repeated(monkeypatch):
+    """Eagerly and within one graph it is handed over; across graphs, or captured after an eager forward pass, it is not."""
+    from style_transfer_amd import token_losses
+    taken = []
+    real = token_losses._take_grad
+    monkeypatch.setattr(token_losses, "_take_grad", lambda *a: taken.append(real(*a)) or taken[-1])
+    x, fns = steps_of(700)
+    side = torch.cuda.Stream()
+    for fn in fns:
+        leaf = x.clone().requires_grad_(True)
+        torch.autograd.grad(fn(leaf), [leaf])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(fn(leaf), [leaf])
+            loss = fn(leaf)
+        torch.cuda.current_stream().wait_stream(side)
+        one, first, second, late = (torch.cuda.CUDAGraph() for _ in range(4))
+        with torch.cuda.graph(late, stream=side):
+            torch.autograd.grad(loss, [leaf])
+        with torch.cuda.graph(one, stream=side):
+            torch.autograd.grad(fn(leaf), [leaf])
+        with torch.cuda.graph(first, stream=side):
+            loss = fn(leaf)
+        with torch.cuda.graph(second, pool=first.pool(), stream=side):
+            torch.autograd.grad(loss, [leaf])
+        assert [for_one for _, for_one in taken] == [1, 1, 0, 1, 0]
+        taken.clear()
