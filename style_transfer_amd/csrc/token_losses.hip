@@ -429,7 +429,7 @@ Split split_of(unsigned rows, int vocab, int size) {
   if (rows < 1024) s = (int)std::min<long long>(MAX_SPLITS, std::min(st::cdivll(1024, std::max(1u, rows)), bytes / 8192));
   s = std::max(1, s);
   const int per = 16 / size;
-  const int chunk = (int)(st::cdivll(st::cdivll(vocab, s), per) * per);
+  const int chunk = (int)std::min<long long>(vocab, st::cdivll(st::cdivll(vocab, s), per) * per);
   return {NT, (int)st::cdivll(vocab, chunk), chunk};
 }
 

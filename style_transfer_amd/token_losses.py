@@ -37,6 +37,7 @@ from . import _lib
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _KINDS = {"sigmoid": 0, "ipo": 1, "hinge": 2}
 _REDUCTIONS = {"token": 0, "sequence": 1}
+_MOST_VOCAB = 2 ** 31 - 1                                       # an int of the C ABI
 
 
 class PreferenceOutput(NamedTuple):
@@ -60,6 +61,8 @@ def _logits_args(x: torch.Tensor):
         raise _lib.StHipError(f"logits: expected fp32, bf16 or fp16, got {x.dtype}")
     if len(shape) not in (2, 3) or shape[-1] == 0:
         raise _lib.StHipError(f"logits: expected [T, V] or [B, L, V], got {tuple(shape)}")
+    if shape[-1] > _MOST_VOCAB:
+        raise _lib.StHipError(f"logits: a vocabulary of {shape[-1]}, at most 2^31 - 1")
     if not x.is_cuda:
         raise _lib.StHipError(f"logits: the HIP hot path needs a tensor on the GPU, got device={x.device} (no CPU fallback)")
     stride = x.stride()

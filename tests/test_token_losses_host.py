@@ -81,3 +81,21 @@ def test_a_loss_without_an_upstream_gradient(nothing_runs, name):
     (_NoGradient.apply(CALLS[name](losses, leaf * 1)) + leaf.sum()).backward()
     if name != "topk_distill_loss":                             # its kernel gets a gradient of 0, and is not there
         assert torch.equal(leaf.grad, torch.ones_like(X))
+
+
+@pytest.mark.parametrize("vocab", [2 ** 31, 2 ** 32 + 5])
+def test_a_vocabulary_beyond_32_bits_is_refused(vocab):
+    """It would reach the kernels as its last 32 bits."""
+    from style_transfer_amd import _lib, losses
+    x, t = torch.empty(1, vocab, dtype=torch.float16, device="meta"), torch.empty(1, dtype=torch.long, device="meta")
+    with pytest.raises(_lib.StHipError, match="at most 2.31 - 1"):
+        losses.token_logprobs(x, t)
+
+
+def test_the_workspace_of_the_largest_vocabulary():
+    """500 rows of 2^31 - 1 elements are cut into parts, a thousand are not: no size on the way wraps."""
+    from style_transfer_amd import _lib
+    lib = _lib.load()
+    plain = lib.st_token_workspace_bytes(1, 1024, 1000, 0)
+    assert lib.st_token_workspace_bytes(1, 1024, 2 ** 31 - 1, 0) == plain
+    assert lib.st_token_workspace_bytes(1, 500, 2 ** 31 - 1, 0) > lib.st_token_workspace_bytes(1, 500, 1000, 0)
