@@ -380,9 +380,9 @@ __device__ __forceinline__ u32x4 gradient_vector(const u32x4& w, const f32x4& k,
   return Type<T>::pack(f);
 }
 
-template <bool PAST, typename V>
-__device__ __forceinline__ void put(V* at, const u32x4& w) {
-  if (PAST) __builtin_nontemporal_store((V)w, at);
+template <bool PAST>
+__device__ __forceinline__ void put(u32x4_u* at, const u32x4& w) {
+  if (PAST) __builtin_nontemporal_store((u32x4_u)w, at);
   else *at = w;
 }
 
