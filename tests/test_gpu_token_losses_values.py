@@ -419,3 +419,48 @@ def test_the_early_gradient_is_used_where_its_forward_pass_is_repeated(monkeypat
             torch.autograd.grad(loss, [leaf])
         assert [for_one for _, for_one in taken] == [1, 1, 0, 1, 0]
         taken.clear()
+
+
+# ---- ordinary rows: how many digits are right -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1000), (torch.bfloat16, 5001), (torch.float32, 32768), (torch.bfloat16, 65536),
+                                         (torch.bfloat16, 131072), (torch.float32, 131072), (torch.bfloat16, 2 ** 20)])
+@pytest.mark.parametrize("lift", [0.0, 8.0, 20.0])
+def test_large_vocabularies_keep_their_digits(dtype, vocab, lift):
+    """A bound that does not grow with the vocabulary.  The roundings of a sum of positive terms are independent, to either side and
+    at most U of what has been added up so far: a thread's n <= 2048 terms are worth at most sqrt(n / 3) U of its share, and T >= 64
+    threads' errors average to 1 / sqrt(T) of that, 3.3 U with n = 2048 and T = 64, less for longer rows, which have more threads;
+    then about 12 joins of U / sqrt(3) each, sqrt(12 / 3) = 2 U, and the exponentials, whose errors average out but for 0.06 U.
+    Five standard deviations of both are 20 U of S, and so 20 U of a log-probability; of the entropy by a factor of its distances
+    from it, which average to H - ln2 sum q d <= 12 nats, weighted like the terms: 3 times as much at most."""
+    from style_transfer_amd.losses import clipped_policy_loss, token_logprobs, topk_distill_loss
+    n = 4
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(n, vocab, generator=g) * 2
+    t = torch.randint(0, vocab, (n,), generator=g)
+    x[torch.arange(n), t] += lift
+    x = x.to(dtype)
+    logp, h, log_q, q = O.token_logprobs(x, t)
+    got, entropy = token_logprobs(x.cuda(), t.cuda(), return_entropy=True)
+    assert bool(((got.cpu().double() - logp).abs() <= 20 * U + U * logp.abs()).all())
+    assert bool(((entropy.cpu().double() - h).abs() <= 60 * U + U * h).all())
+    # each row alone, so that nothing averages: the ratio is 1, its error the log-probability's
+    for r in range(n):
+        leaf = x[r:r + 1].cuda().requires_grad_(True)
+        old = logp[r:r + 1].float()
+        loss, stats = clipped_policy_loss(leaf[None], t[r:r + 1][None].cuda(), old[None].cuda(), -torch.ones(1, 1).cuda())
+        loss.backward()
+        ratio = math.exp(float(logp[r]) - float(old))
+        assert abs(float(stats[0]) - ratio) <= 22 * U and abs(float(stats[2]) - float(h[r])) <= 60 * U + U * float(h[r])
+        # an entry: 20 U of S, its own exponent of up to 32 bits, a few roundings; at the label 1 - q is left of both
+        want = O.row_gradient(t[r:r + 1], 1.0, h, log_q[r:r + 1], q[r:r + 1], torch.tensor([ratio], dtype=torch.float64), torch.zeros(1))[0]
+        half = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}[dtype]
+        bound = want.abs() * half + 50 * U * ratio * q[r]
+        bound[t[r]] += 4 * U
+        assert bool(((leaf.grad[0].cpu().double() - want).abs() <= bound + 2.0 ** -126).all())
+        if vocab <= 131072:
+            idx = torch.stack([t[r], (t[r] + 1) % vocab])[None]
+            val = torch.tensor([[-0.25, -2.0]])
+            for tail in (False, True):
+                want, _ = O.distill(x[r:r + 1], idx, val, None, 1.0, tail)
+                got = topk_distill_loss(x[r:r + 1].cuda(), idx.cuda(), val.cuda(), tail=tail)
+                assert abs(float(got) - want) <= 40 * U + U * abs(want)
