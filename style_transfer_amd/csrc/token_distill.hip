@@ -180,12 +180,24 @@ struct Unlisted {
   __device__ __forceinline__ float extra(int t, float v) const { return t < 32 && marks.bits[last] >> t & 1 ? -INFINITY : v; }
 };
 
+// exp((v - vref) / tau) with the exponent in two numbers, so that it has no rounding: what the difference leaves, and what c (with
+// c_lo) leaves of log2(e) / tau.  Most of a gradient's norm is in the listed entries; in 64 bits this is 6 to 15 % of the time of
+// short rows (65536 of 1000 bf16, 16384 of 4096).
+__device__ __forceinline__ float listed_mass(float v, float vref, float c, float c_lo) {
+#pragma clang fp contract(off)
+  const float t = v - vref, back = t - v, left = (v - (t - back)) - (vref + back);
+  const float y = t * c, k = rintf(y);
+  if (y < D_MIN) return 0.f;
+  return ldexpf(__builtin_amdgcn_exp2f(fmaf(t, c, -k) + fmaf(left, c, t * c_lo)), (int)k);
+}
+
 // The entries of a row's list that lie in [lo, lo + n), over the stream that wrote them as if they were off it: entry t of
 // each thread (in `mine`), t + threads, ...  x and out are the row's beginning.
 template <typename T>
 __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, unsigned r, const f32x4& a, const f32x4& b, float scale, int lo,
                                            int n, const T* x, T* out, const Entry<T>& mine, int t, int threads) {
-  const float cv = q.tail ? (float)(1.0 / LN2) : p.c;
+  const double log2e = (q.tail ? 1.0 : p.inv_tau) * (1.0 / LN2);
+  const float cv = (float)log2e, cv_lo = (float)(log2e - (double)cv);
   const Ref ref = make_ref(a[2], p.c);
   const size_t first = (size_t)r * q.k;
   Entry<T> e = mine;
@@ -194,9 +206,9 @@ __device__ __forceinline__ void patch_list(const Logits& p, const ListIn& q, uns
       float pk = 0.f;
       if (b[2] != 0.f) {                                        // an index twice in this row: its entries' sum, in order
         for (int i = 0; i < q.k; ++i)
-          if (entry_index(q, first + i, p.vocab) == e.j) pk += __builtin_amdgcn_exp2f((q.val[first + i] - b[0]) * cv);
+          if (entry_index(q, first + i, p.vocab) == e.j) pk += listed_mass(q.val[first + i], b[0], cv, cv_lo);
       } else {
-        pk = __builtin_amdgcn_exp2f((e.v - b[0]) * cv);
+        pk = listed_mass(e.v, b[0], cv, cv_lo);
       }
       const float ex = __builtin_amdgcn_exp2f(distance((float)e.x, ref, p.c));
       out[e.j] = (T)(scale * (a[3] * ex - b[1] * pk));

@@ -464,3 +464,27 @@ def test_large_vocabularies_keep_their_digits(dtype, vocab, lift):
                 want, _ = O.distill(x[r:r + 1], idx, val, None, 1.0, tail)
                 got = topk_distill_loss(x[r:r + 1].cuda(), idx.cuda(), val.cuda(), tail=tail)
                 assert abs(float(got) - want) <= 40 * U + U * abs(want)
+
+
+@pytest.mark.parametrize("vocab,k,tail,tau", [(1000, 40, True, 1.0), (20000, 300, True, 1.7), (9000, 40, False, 1.7), (60000, 1500, False, 1.0)])
+def test_distill_listed_entries_have_the_digits_of_their_probabilities(vocab, k, tail, tau):
+    """Listed entries are tau (Q q_j - p_j) over the rows, however far apart the values are: p_j within 6 U, since its exponent is a
+    whole number and a fraction of at most 1/2 (0.4 U), the exponential is within 2 U, the row's coefficient, the product and the
+    entry are rounded; q_j, with an exponent of up to 32 bits that is rounded once, within 20 U of S as any row's, 22 U and 6 U."""
+    from style_transfer_amd.losses import topk_distill_loss
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(2, vocab, generator=g) * 4
+    idx = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(2)])
+    val = torch.randn(2, k, generator=g) * 4
+    if tail:
+        val = torch.log_softmax(val, 1) - 0.05
+    _, want = O.distill(x, idx, val, None, tau, tail)
+    leaf = x.cuda().requires_grad_(True)
+    loss = topk_distill_loss(leaf, idx.cuda(), val.cuda(), temperature=tau, tail=tail)
+    got, = torch.autograd.grad(loss, [leaf], retain_graph=True)
+    again, = torch.autograd.grad(loss, [leaf])                  # computed from the saved coefficients
+    q = torch.stack([O.row(r, tau)[1] for r in x])
+    p = (val.double() if tail else torch.log_softmax(val.double() / tau, 1)).exp()
+    bound = tau / 2 * (q.gather(1, idx) * 48 * U + p * 6 * U) + 2.0 ** -126
+    assert torch.equal(got, again)
+    assert bool(((got.cpu().double() - want).gather(1, idx).abs() <= bound).all())
