@@ -251,9 +251,10 @@ def _keep(ctx, grad, *tensors):
 
 
 def _capture(x):
-    """The graph that is being captured, 0 outside of a capture."""
+    """The graph that is being captured, 0 outside of a capture, and on the null stream, which cannot be captured."""
     with _on(x):
-        return _lib.load().st_capture_id(_lib.stream_ptr())
+        stream = _lib.stream_ptr()
+    return _lib.load().st_capture_id(stream) if stream else 0
 
 
 def _take_grad(ctx, x, early):
