@@ -18,7 +18,8 @@ namespace {
 using namespace st_token;
 
 constexpr int MAX_VOCAB = 1 << 20;       // the bitmap of a row: 128 KB of LDS
-constexpr int MAX_LIST = 4096;           // a list that names a token twice is gone through once for each entry
+constexpr int MAX_LIST = 4096;           // a list that names a token twice is gone through once for each entry: 1024 rows of 32768
+                                         // bf16, value and gradient, 132 -> 188 us with K = 256, 0.12 -> 1.8 ms with 1024, 0.23 -> 28 ms with 4096
 constexpr size_t MAX_PLAIN_LDS = 48 << 10;   // dynamic LDS that a kernel gets without asking (64 KB with what it declares)
 
 // what the list of a row, or a wave's part of it, says by itself
@@ -303,9 +304,9 @@ __device__ __forceinline__ bool sync_row_or(bool v) {
   return __any(v);
 }
 
-// The logits are read once and the gradient written once: 4096 rows of 32768 bf16, K = 64, in 106 us, 5.1 TB/s (what a copy
-// reaches); of 131072 in 463 us, 4.6 TB/s, where one row fills a compute unit and its reading and writing take turns; 1024 rows of
-// 131072 fp32, of which the last 192 KB each are read twice, in 242 us, 4.4 TB/s.
+// The logits are read once and the gradient written once: 4096 rows of 32768 bf16, K = 64, in 122 us, 4.4 TB/s (a copy reaches
+// 6.4); of 131072 in 507 us, 4.2 TB/s, where one row fills a compute unit and its reading and writing take turns; 1024 rows of
+// 131072 fp32, of which the last 192 KB each are read twice (K = 256: 200 MB of that from beyond the L2), in 251 us, 4.3 TB/s.
 template <typename T, typename S>
 __global__ __launch_bounds__(S::BLOCK, 4) void distill_kernel(Logits p, ListIn q, Sums u, int words, T* __restrict__ grad) {
   constexpr int TPR = S::TPR, VEC = Type<T>::VEC;

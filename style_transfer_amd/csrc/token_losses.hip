@@ -83,7 +83,7 @@ __device__ __forceinline__ Part stream_part(const T* x, int n, float c, int t) {
 }
 
 // One read of the logits, a running reference a thread, no more than a few floats written a row: 4096 rows of 131072 bf16 in
-// 186 us, 5.8 TB/s (a copy reaches 5.1, reading and writing); one such row, cut into 32 parts, with join_kernel in 6 us.
+// 175 us, 6.1 TB/s (a kernel that only reads reaches 7.2); one such row, cut into 32 parts, with join_kernel in 6 us.
 template <typename T, int TPR, bool KEEP>
 __global__ __launch_bounds__(NT) void stats_kernel(Logits p, int splits, int chunk, StatsOut o) {
   __shared__ Part red[NT / 64];
@@ -155,7 +155,8 @@ __device__ __forceinline__ RowGrad row_grad(const Logits& p, const GradIn& g, un
   return v;
 }
 
-// Reads the logits again and writes the gradient, 16 KB a block: 4096 rows of 131072 bf16 in 366 us, 5.9 TB/s.
+// Reads the logits again and writes the gradient, 16 KB a block: 4096 rows of 131072 bf16 in 357 us, 6.0 TB/s
+// (a copy reaches 6.4).
 template <typename T, int TPR>
 __global__ __launch_bounds__(NT) void grad_kernel(Logits p, GradIn g, int splits, int chunk, T* __restrict__ grad) {
   const float scale = g.gout ? g.gout[0] : 1.f;
@@ -354,10 +355,10 @@ __global__ __launch_bounds__(1024) void count_kernel(Logits p, PolicyIn q, Sums 
 }
 
 // One pass: a row's statistics, its terms and, where the caller wants one, its gradient (for an upstream gradient of 1).  With
-// the row in registers the logits are read once: 4096 rows of 131072 bf16 in 415 us, 5.2 TB/s read and written (two passes would take
-// 552), of 32768 in 101 us, 5.3 TB/s; 1024 rows of 131072 fp32, of which the last 192 KB each are read twice, in 237 us, 4.5 TB/s.
-// Rows of 2 KB are bound by what a wave does once a row (65536 of 1000 bf16: 73 us, 3.6 TB/s; 78 before the row's number was in a
-// scalar register).
+// the row in registers the logits are read once: 4096 rows of 131072 bf16 in 412 to 452 us, 4.8 to 5.2 TB/s read and written (two passes
+// take 532), of 32768 in 111 us, 4.9 TB/s; 1024 rows of 131072 fp32, of which the last 192 KB each are read twice, in 254 us, 4.2 TB/s.
+// Rows of 2 KB are bound by what a wave does once a row (65536 of 1000 bf16: 79 us, 3.3 TB/s; 5 us of them for a row's
+// logarithm, ratio and estimate in 64 bits).
 template <typename T, typename S>
 __global__ __launch_bounds__(S::BLOCK, 4) void policy_kernel(Logits p, PolicyIn q, Sums u, T* __restrict__ grad) {
   constexpr int TPR = S::TPR;

@@ -10,19 +10,19 @@
 //
 // m is a value near the maximum, not the maximum itself: a wave takes the largest of its first vector and another one where an
 // element lies more than a bit above it.  That saves a pass over the row, and lets the exponentials begin while the row is
-// still arriving; and since no d_j is above 1.5, the elements that S consists of have an exponent without error.  (With the
-// first reference kept as long as S stays below 2^80 a dominant element's d_j reaches 80, whose rounding is 2.6e-6 of S.)  m c
-// is rounded to a whole number, which then stands for the reference everywhere: d_j is one fused multiply-add with no error but
-// its own, and a part seen from another reference is multiplied by a power of two, exactly.  (The hardware's exponential is 3.4e-9 too small on average, and an element would go
-// through four of them on its way into S.)
+// still arriving; and since no d_j is above 1.5, the elements that S mostly consists of have hardly any rounding in their
+// exponents.  (With the first reference kept as long as S stays below 2^80 a dominant element's d_j reaches 80, whose rounding is
+// 2.6e-6 of S.)  m c is rounded to a whole number, which then stands for the reference everywhere: d_j is one fused multiply-add
+// with no error but its own, and a part seen from another reference is multiplied by a power of two, exactly.  (The hardware's
+// exponential is 3.4e-9 too small on average, and an element would go through four of them on its way into S.)
 //
 // Where |m c| reaches 2^24 ("low" rows: nothing but a mask's value, -1e9 or the lowest of the type) the next whole number can be
 // far from it, and the difference comes first, d_j = (x_j - m) c: such a row is the uniform distribution that the formula gives,
 // whatever the value.  A row of -inf only has S = 0: no distribution, log-probability -inf, entropy 0, gradient 0.
 //
-// Sums of a row are fp32 per thread and over a fixed tree; what a row is reduced to is finished around fp64 sums (one wave a
-// row), because a sequence's sum of hundreds of log-probabilities is compared with another model's: c's own rounding
-// (relative 2^-25) shifts every term the same way, and W, which is d S / d ln c up to a factor, takes that shift out again.
+// Sums of a row are fp32 per thread and over a fixed tree; what a row is reduced to is finished in fp64 (one wave a row),
+// because a sequence's sum of hundreds of log-probabilities is compared with another model's: c's own rounding (relative 2^-24
+// at most) shifts every term the same way, and W, which is d S / d ln c up to a factor, takes that shift out again.
 #pragma once
 #include <algorithm>
 #include <cmath>

@@ -20,7 +20,8 @@ What they have in common:
 * ``clipped_policy_loss`` and ``topk_distill_loss`` write the gradient of logits that require one in the forward pass, while
   a row is on chip.  A backward pass with an upstream gradient of 1 hands it over; another one (a loss weight outside, a
   dynamic loss scale) computes it again from the logits: pass a known factor as ``scale``.  Until then it is a saved tensor of
-  the logits' size beside them, and goes where saved tensors go.
+  the logits' size beside them, and goes where saved tensors go.  Captured into another graph than its forward pass, a backward
+  pass always computes it again.
 """
 from __future__ import annotations
 
@@ -383,7 +384,8 @@ def clipped_policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: t
                         clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
                         reduction: str = "token", ignore_index: int = -100, scale: float = 1.0) -> PolicyOutput:
     """Clipped policy loss of sampled tokens.  With ``logp`` the label's log-probability, ``r = exp(logp - old_logps)`` and ``A``
-    the advantage (the labels' shape: of each position; else ``[sequences]``: one for all of a sequence), a position's loss is
+    the advantage (the labels' shape: of each position, also where a packed batch has as many sequences as rows; else
+    ``[sequences]``: one for all of a sequence), a position's loss is
 
     ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - logp) - (ref - logp) - 1) - entropy_coef H``
 
@@ -463,8 +465,9 @@ def topk_distill_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     they are the teacher's log-probabilities (at ``temperature``, over its whole vocabulary), and all tokens that are not listed
     form one more entry of the sum, with ``1 - sum_k p_k`` and the student's probability of the same tokens.
 
-    At most 2^20 tokens and 4096 entries.  A position with no used entry contributes 0.  An index of ``V`` or more makes its position's loss and
-    gradient NaN."""
+    At most 2^20 tokens and 4096 entries.  A position with no used entry contributes 0.  An index of ``V`` or more makes its position's
+    loss and gradient NaN.  Fill a short list up with -1, not by naming a token again: such a list costs the square of its length (1024
+    positions of 32768 tokens: 0.2 ms instead of 0.13 with 256 entries, 28 instead of 0.23 with 4096)."""
     args = _logits_args(logits)
     shape = logits.shape[:-1]
     if not isinstance(teacher_indices, torch.Tensor) or teacher_indices.dim() != logits.dim() or teacher_indices.shape[-1] == 0:
