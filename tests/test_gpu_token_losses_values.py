@@ -488,3 +488,72 @@ def test_distill_listed_entries_have_the_digits_of_their_probabilities(vocab, k,
     bound = tau / 2 * (q.gather(1, idx) * 48 * U + p * 6 * U) + 2.0 ** -126
     assert torch.equal(got, again)
     assert bool(((got.cpu().double() - want).gather(1, idx).abs() <= bound).all())
+
+
+# ---- rows in which the reference moves -------------------------------------------------------------------------------------------------
+def moving_rows(dtype, vocab):
+    """Rising, falling, stepping up and down, up from a mask, into the low range at the end or in one element, past it and back."""
+    up = torch.linspace(-60, 60, vocab)
+    x = torch.stack([up, up.flip(0), torch.where(torch.arange(vocab) % 512 < 256, up, -up), up, up, up / 60])
+    x[2] += 0.25 * torch.randn(vocab, generator=torch.Generator().manual_seed(vocab))
+    x[3, : vocab * 3 // 4] = -INF
+    if dtype != torch.float16:
+        x[4, vocab - 3:] = 3e7
+        x[5, vocab // 2] = 2.5e7
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype,vocab", ROWS + [(torch.bfloat16, 170001), (torch.float32, 90000)])
+def test_rows_in_which_the_reference_moves(dtype, vocab):
+    from style_transfer_amd.losses import clipped_policy_loss, topk_distill_loss
+    x = moving_rows(dtype, vocab)
+    n = x.shape[0]
+    t = torch.tensor([vocab - 1, 0, vocab - 1, vocab - 2, vocab - 1, vocab // 2])
+    logp, h, log_q, q = O.token_logprobs(x, t)
+    row = (vocab / 64 + 64) * U
+    half, tiny = {torch.float32: (U, 2.0 ** -126), torch.bfloat16: (2.0 ** -8, 2.0 ** -126), torch.float16: (2.0 ** -11, 2.0 ** -25)}[dtype]
+    for r in range(n):
+        leaf = x[r:r + 1].cuda().requires_grad_(True)
+        old = logp[r:r + 1].float()
+        loss, stats = clipped_policy_loss(leaf[None], t[r:r + 1][None].cuda(), old[None].cuda(), -torch.ones(1, 1).cuda(), entropy_coef=0.1)
+        loss.backward()
+        ratio = math.exp(float(logp[r]) - float(old))
+        assert abs(float(stats[0]) - ratio) <= row + 2 * U
+        assert abs(float(stats[2]) - float(h[r])) <= (float(h[r]) + 2) * row + 2 * U * float(h[r])
+        a, b = torch.tensor([ratio], dtype=torch.float64), torch.tensor([-0.1], dtype=torch.float64)
+        want = O.row_gradient(t[r:r + 1], 1.0, h[r:r + 1], log_q[r:r + 1], q[r:r + 1], a, b)
+        low = log_q[r].clamp(min=-200.0).abs()
+        # as any row's: S, the exponent of an entry, roundings; and the exponential is 0 below 2^-126, an entry this many times that
+        size = ratio + 0.1 * (low + h[r])
+        fp32 = q[r] * size * (row + 10 * U + 3 * low * U) + size * 2.0 ** -126
+        fp32[t[r]] += 8 * U
+        assert bool(((leaf.grad.cpu().double() - want)[0].abs() <= (want[0].abs() + fp32) * half * 1.01 + fp32 + tiny).all()), r
+        idx, val = torch.tensor([[int(t[r]), vocab // 2 + 1, vocab - 5]]), torch.tensor([[-0.5, -2.0, -2.5]])
+        val = val.masked_fill(x[r].gather(0, idx[0])[None] == -INF, -INF)
+        for tail in (False, True):
+            want_loss, want = O.distill(x[r:r + 1], idx, val, None, 1.0, tail)
+            leaf.grad = None
+            got = topk_distill_loss(leaf, idx.cuda(), val.cuda(), tail=tail)
+            got.backward()
+            # p (log p - log q): q is up to e^-120, or e^-3e7, of which fp32 keeps 2 U
+            assert abs(float(got.detach()) - want_loss) <= 2 * row + 60 * U + abs(want_loss) * 4 * U
+            fp32 = (2 * q[r] + (want[0] - q[r]).abs()) * (2 * row + 40 * U + 6 * low * U)
+            assert bool(((leaf.grad.cpu().double() - want)[0].abs() <= (want[0].abs() + fp32) * half * 1.01 + fp32 + tiny).all()), r
+
+
+@pytest.mark.parametrize("dtype,vocab", ROWS)
+@pytest.mark.parametrize("value", [INF, math.nan])
+def test_a_value_without_a_softmax_anywhere_in_a_row(dtype, vocab, value):
+    """+inf or NaN in the first vector, in the middle or outside the vectors: the row is NaN, and no other."""
+    from style_transfer_amd.losses import clipped_policy_loss
+    x = torch.randn(4, vocab, generator=torch.Generator().manual_seed(1)).to(dtype)
+    for r, at in enumerate((1, vocab // 2, vocab - 1)):
+        x[r, at] = value
+    leaf = x.cuda().requires_grad_(True)
+    t = torch.tensor([[5, 6, 7, 8]]).cuda()
+    for r in range(4):
+        loss, stats = clipped_policy_loss(leaf[None, r:r + 1], t[:, r:r + 1], torch.full((1, 1), -9.0).cuda(), -torch.ones(1, 1).cuda(), clip_low=0.0)
+        assert math.isnan(float(stats[2])) == (r < 3)
+    old = torch.full((1, 4), -9.0).cuda()
+    clipped_policy_loss(leaf[None], t, old, -torch.ones(1, 4).cuda(), clip_low=0.0, entropy_coef=0.1).loss.backward()
+    assert torch.isnan(leaf.grad[:3]).all() and torch.isfinite(leaf.grad[3]).all()
