@@ -244,25 +244,23 @@ def _wants_grad(x: torch.Tensor) -> bool:
 
 
 # ---- the two losses whose rows go through the label's log-probability -------------------------------------------------------------
-def _keep(ctx, grad, *tensors):
+def _keep(ctx, grad, capture, *tensors):
     """Saves what the backward pass reads, the gradient that the forward kernel wrote among it, so that saved-tensor hooks (the
     host's memory, a checkpoint) reach it too.  ``data``: with a version of its own, since it is given away and may be changed."""
-    ctx.given, ctx.capture = False, _capture(grad)
+    ctx.given, ctx.capture = False, capture
     ctx.save_for_backward(*tensors, grad.data)
 
 
-def _capture(x):
+def _capture(lib, stream):
     """The graph that is being captured, 0 outside of a capture, and on the null stream, which cannot be captured."""
-    with _on(x):
-        stream = _lib.stream_ptr()
-    return _lib.load().st_capture_id(stream) if stream else 0
+    return lib.st_capture_id(stream) if stream else 0
 
 
-def _take_grad(ctx, x, early):
+def _take_grad(ctx, x, early, capture):
     """(buffer, 1) the first time: it holds the gradient for an upstream gradient of 1, written by the forward kernel while the
     rows were on chip.  The buffer is given away, so a second backward pass gets a new one, (buffer, 0); as does one that is
     captured without its forward pass, since its replays would find in the buffer what the last of them left."""
-    if ctx.given or not early or ctx.capture != _capture(x):
+    if ctx.given or not early or ctx.capture != capture:
         return _grad_buffer(x), 0
     ctx.given = True
     return early[0].data, 1
@@ -273,10 +271,12 @@ def _token_loss_bwd(ctx, gout):
         return None, None
     x, labels, row_grad, *early = ctx.saved_tensors
     args, tau, ignore = ctx.call
-    grad, for_one = _take_grad(ctx, x, early)
+    lib = _lib.load()
     with _on(x):
-        _lib.check(_lib.load().st_token_loss_bwd(*_place(x, args), *_label_args(labels, ignore), tau, row_grad.data_ptr(), gout.data_ptr(), for_one,
-                                                 grad.data_ptr(), _lib.stream_ptr()), "st_token_loss_bwd")
+        stream = _lib.stream_ptr()
+        grad, for_one = _take_grad(ctx, x, early, _capture(lib, stream))
+        _lib.check(lib.st_token_loss_bwd(*_place(x, args), *_label_args(labels, ignore), tau, row_grad.data_ptr(), gout.data_ptr(), for_one,
+                                         grad.data_ptr(), stream), "st_token_loss_bwd")
     return grad, None
 
 
@@ -356,22 +356,23 @@ def _policy_fwd(x, call, need):
     loss, stats = _f32(x), _f32(x, 4)
     grad = _grad_buffer(x) if need else None
     with _on(x):
+        stream = _lib.stream_ptr()
         buffer, row_grad, work = _scratch(x, 16 * rows if need else 0, lib.st_token_workspace_bytes(args[1], rows, args[6], sequences))
         _lib.check(lib.st_policy_loss_fwd(*args, *_label_args(labels, ignore), tau, _ptr(cu), sequences, old.data_ptr(), adv.data_ptr(),
                                           int(adv.shape != labels.shape), _ptr(ref), low, high, kl, ent, per_sequence, scale,
-                                          loss.data_ptr(), stats.data_ptr(), row_grad if need else None, _ptr(grad), work,
-                                          _lib.stream_ptr()), "st_policy_loss_fwd")
-    return loss, stats, grad, buffer
+                                          loss.data_ptr(), stats.data_ptr(), row_grad if need else None, _ptr(grad), work, stream),
+                   "st_policy_loss_fwd")
+    return loss, stats, grad, buffer, _capture(lib, stream)
 
 
 class _PolicyFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        loss, stats, grad, buffer = _policy_fwd(x, call, True)
+        loss, stats, grad, buffer, capture = _policy_fwd(x, call, True)
         ctx.mark_non_differentiable(stats)
         ctx.set_materialize_grads(False)
         ctx.call = call[0], call[3], call[2]
-        _keep(ctx, grad, x, call[1], buffer)
+        _keep(ctx, grad, capture, x, call[1], buffer)
         return loss, stats
 
     @_backward
@@ -427,29 +428,31 @@ def _distill_fwd(x, call, need):
     grad = _grad_buffer(x) if need else None
     entries = (idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1])
     with _on(x):
+        stream = _lib.stream_ptr()
         buffer, row_grad, work = _scratch(x, 32 * rows if need else 0, lib.st_distill_workspace_bytes(rows))
         _lib.check(lib.st_distill_loss_fwd(*args, *entries, _ptr(mask), tau, tail, scale, loss.data_ptr(), row_grad if need else None,
-                                           _ptr(grad), work, _lib.stream_ptr()), "st_distill_loss_fwd")
-    return loss, grad, buffer
+                                           _ptr(grad), work, stream), "st_distill_loss_fwd")
+    return loss, grad, buffer, _capture(lib, stream)
 
 
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        loss, grad, buffer = _distill_fwd(x, call, True)
+        loss, grad, buffer, capture = _distill_fwd(x, call, True)
         ctx.call = call[0], call[4], call[5]
-        _keep(ctx, grad, x, call[1], call[2], buffer)
+        _keep(ctx, grad, capture, x, call[1], call[2], buffer)
         return loss
 
     @_backward
     def backward(ctx, gout):
         x, idx, val, row_grad, *early = ctx.saved_tensors
         args, tau, tail = ctx.call
-        grad, for_one = _take_grad(ctx, x, early)
+        lib = _lib.load()
         with _on(x):
-            _lib.check(_lib.load().st_distill_loss_bwd(*_place(x, args), idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1], tau, tail,
-                                                       row_grad.data_ptr(), gout.data_ptr(), for_one, grad.data_ptr(), _lib.stream_ptr()),
-                       "st_distill_loss_bwd")
+            stream = _lib.stream_ptr()
+            grad, for_one = _take_grad(ctx, x, early, _capture(lib, stream))
+            _lib.check(lib.st_distill_loss_bwd(*_place(x, args), idx.data_ptr(), int(idx.dtype is torch.int64), val.data_ptr(), idx.shape[-1], tau, tail,
+                                               row_grad.data_ptr(), gout.data_ptr(), for_one, grad.data_ptr(), stream), "st_distill_loss_bwd")
         return grad, None
 
 
